@@ -581,6 +581,117 @@ int sv2_inner_product_f16_few(const void* x, const void* w, const void* w_value,
 int sv2_inner_product_f32(const float* x, const float* w, const float* bias, float* y, int rows, int in, int out,
                           void* stream);
 
+/* ------------------------------------------------------------------------
+ * Operators around the DiT blocks for clips of many frames: attention of a
+ * chunk of tokens over a cache, group normalisation of a channels-last video
+ * (the reference's DynamicFramewiseGroupNorm, src/layers/
+ * dynamic_framewise_group_norm.cpp:62-143, with the activation that follows
+ * it) and matrix products with their epilogues.  Strides are in elements;
+ * the last dimension of every tensor is contiguous.  Outputs must not overlap
+ * inputs except where said.
+ * ------------------------------------------------------------------------ */
+
+/* Activations, in fp32: v; v / (1 + exp(-v)); v/2 (1 + erf(v / sqrt 2));
+ * v/2 (1 + tanh(sqrt(2/pi) (v + 0.044715 v^3))). */
+typedef enum sv2_activation {
+    SV2_ACT_NONE = 0,
+    SV2_ACT_SILU = 1,
+    SV2_ACT_GELU = 2,
+    SV2_ACT_GELU_TANH = 3
+} sv2_activation;
+
+/* Attention of q_len query tokens over kv_len cached tokens, with a sliding
+ * window and first tokens that stay visible.  Sequence b has nq = q_lens[b]
+ * queries and nk = kv_lens[b] keys (the sizes themselves where the array is
+ * NULL; values outside 0 .. size count as the nearest bound); its query i is
+ * the token at position p = nk - nq + i and sees key j where
+ *     j < nk,  j <= p + right,  and  j < sinks or j >= p - left
+ * (right = 0: causal; left and right INT_MAX: everything).
+ *     out = sum_j softmax_j(scale q.k_j) v_j over the visible keys.
+ * A query that sees no key gets 0 (lse -infinity); so does one whose visible
+ * scores are all -infinity.  Rows i >= nq of out and lse are left as they
+ * were.  Keys and values that no query of the sequence sees may hold
+ * anything; what a query does not see does not reach its output. */
+typedef struct sv2_sliding_attn_args {
+    int batch;
+    int q_len, kv_len;   /* sizes of the token dimension of q / out and k / v */
+    int heads, kv_heads; /* query head h reads key head h / (heads / kv_heads) */
+    int head_dim;        /* 64 or 128 */
+    int dtype;           /* SV2_F16 or SV2_BF16: q, k, v and out */
+    int left, right, sinks;
+    float scale;         /* > 0 */
+    const void* q;       /* [batch][q_len][heads][head_dim] by the strides below */
+    int64_t q_batch_stride, q_token_stride, q_head_stride;
+    const void* k;       /* [batch][kv_len][kv_heads][head_dim] */
+    int64_t k_batch_stride, k_token_stride, k_head_stride;
+    const void* v;
+    int64_t v_batch_stride, v_token_stride, v_head_stride;
+    void* out;           /* as q */
+    int64_t out_batch_stride, out_token_stride, out_head_stride;
+    const int32_t* q_lens;  /* device [batch] or NULL; read when the kernels run, so */
+    const int32_t* kv_lens; /* a captured call follows lengths written before a replay */
+    float* lse;          /* device [batch][heads][q_len] or NULL: ln sum_j exp(scale q.k_j) */
+    void* workspace;     /* device, sv2_sliding_attention_workspace() bytes; not shared by */
+    size_t workspace_bytes; /* calls that may overlap */
+} sv2_sliding_attn_args;
+
+/* Host.  Device workspace bytes of a call with these sizes (its pointers,
+ * strides and lengths do not matter), or a negative error code. */
+int64_t sv2_sliding_attention_workspace(const sv2_sliding_attn_args* args);
+
+/* Device.  The attention above.  q, k, v, out and the workspace must be
+ * 16-byte aligned and every stride a multiple of 8 elements (SV2_EINVAL);
+ * token strides of k and v up to 2^24 elements, head_dim 64 or 128
+ * (SV2_EUNSUPPORTED).  Results do not depend on timing. */
+int sv2_sliding_attention(const sv2_sliding_attn_args* args, void* stream);
+
+/* Host.  Device workspace bytes of sv2_group_norm, or a negative error code. */
+int64_t sv2_group_norm_workspace(int dtype, int images, int rows, int channels, int groups);
+
+/* Device.  Group normalisation and activation of `images` images (frames) of
+ * `rows` pixels of `channels` channels, channels last:
+ *     y = act((x - mean) / sqrt(var + eps) * gamma[c] + beta[c])
+ * mean and biased variance per image and group of channels / groups
+ * consecutive channels, over all its rows.  x, y of dtype (fp32, fp16, bf16);
+ * statistics and gamma, beta (fp32 [channels], NULL: 1 and 0) in fp32.  y may
+ * be x (with the same strides).  Any alignment and strides; 16-byte aligned
+ * tensors with strides and channels in multiples of 16 bytes are several times
+ * as fast.  Row strides are at least `channels`; more than 8192 channels give
+ * SV2_EUNSUPPORTED.  Calls that share a workspace must not overlap. */
+int sv2_group_norm(const void* x, int64_t x_image_stride, int64_t x_row_stride, void* y, int64_t y_image_stride,
+                   int64_t y_row_stride, int dtype, int images, int rows, int channels, int groups, float eps,
+                   const float* gamma, const float* beta, int activation, void* workspace, size_t workspace_bytes,
+                   void* stream);
+
+/* y [rows, out] = act(x [rows, in] W^T + bias) + residual, W [out, in]; x, W,
+ * y and residual of dtype, sums and bias in fp32, one rounding at the end.
+ * bias and residual may be NULL; y may be the residual (with its stride). */
+typedef struct sv2_linear_args {
+    int rows, in, out;
+    int dtype;      /* SV2_F16 or SV2_BF16 (fp32 products: sv2_inner_product_f32) */
+    int activation; /* sv2_activation */
+    const void* x;
+    int64_t x_stride; /* elements between rows, at least `in` */
+    const void* w;
+    int64_t w_stride;
+    const float* bias; /* [out] */
+    const void* residual;
+    int64_t residual_stride;
+    void* y;
+    int64_t y_stride;
+    void* workspace; /* device, sv2_linear_workspace() bytes, 16-byte aligned; not shared by calls that may overlap */
+    size_t workspace_bytes;
+} sv2_linear_args;
+
+/* Host.  Device workspace bytes of a call with these sizes (its pointers and
+ * strides do not matter), or a negative error code. */
+int64_t sv2_linear_workspace(const sv2_linear_args* args);
+
+/* Device.  The product above; any sizes, strides and element alignment.
+ * Operands that are 16-byte aligned with row strides of a multiple of 8
+ * elements run on the faster kernels. */
+int sv2_linear(const sv2_linear_args* args, void* stream);
+
 /* ---- Euler sampler (src/model/sampler.h:18-78) and the latent preparation
  * of the engine loop (src/core/engine.cpp:79-149, :306-350).  Latents are
  * fp32 device arrays treated as flat element sequences except where a layout

@@ -1,0 +1,661 @@
+// Group normalisation with its activation, channels last.
+//
+//   y[i][r][c] = act((x[i][r][c] - mean) / sqrt(var + eps) * gamma[c] + beta[c])
+//
+// with the mean and the biased variance of image i over all rows and the
+// `width` channels of c's group.  Memory-bound: 16 bytes per lane per access
+// where the layout allows them (V elements, else one).
+//
+// Statistics.  Every thread keeps V fixed channels and walks rows; it forms
+// the mean and the sum of squared differences of a few rows held in registers
+// in two passes, and joins such pieces pairwise (n, mean, M2), so that no
+// difference of large sums is taken however far the mean is from zero.  The
+// pieces of a workgroup are joined per group through LDS the same way: the
+// weighted mean first (as differences from one of the means), then
+// M2 + n (mean_i - mean)^2.  All of it in a fixed order: the same input gives
+// the same output.
+//
+// Two forms, by the size of an image.
+//   slab   a workgroup holds the rows of some whole groups of an image in
+//          registers (128 KB at most): one launch, x read once.
+//   rows   three launches: every workgroup reduces a run of rows, a small
+//          kernel joins the runs, and a last pass reads x again.
+#include "sv2_internal.h"
+#include "activation.h"
+#include "vec_io.h"
+
+#include <algorithm>
+#include <climits>
+#include <type_traits>
+
+namespace sv2
+{
+namespace
+{
+
+using namespace vec;
+
+struct NormArgs
+{
+    const void* x;
+    void* y;
+    long long x_image, x_row, y_image, y_row; // strides in elements
+    const float* gamma;
+    const float* beta;
+    int rows, channels, groups, width;
+    float eps;
+    int slab_groups, slabs;   // slab form
+    int chunk_rows, chunks;   // rows form
+    float2* part;             // rows form: (mean, M2) [image][group][chunk], then (mean, rstd) [image][group]
+    float2* stat;
+};
+
+constexpr int kSlabThreads = 1024;
+constexpr int kRowThreads = 256;
+constexpr int kMaxChannels = 8192;
+
+template <typename T>
+constexpr int elem_bytes()
+{
+    return std::is_same_v<T, F32> ? 4 : 2;
+}
+
+// V elements of one row piece, as loaded.
+template <typename T, int V>
+struct Piece;
+template <typename T>
+struct Piece<T, 1>
+{
+    float v;
+    __device__ void load(const void* base, long long i)
+    {
+        if constexpr (std::is_same_v<T, F32>)
+            v = static_cast<const float*>(base)[i];
+        else if constexpr (std::is_same_v<T, F16>)
+            v = static_cast<float>(static_cast<const _Float16*>(base)[i]);
+        else
+            v = __builtin_bit_cast(float, static_cast<uint32_t>(static_cast<const uint16_t*>(base)[i]) << 16);
+    }
+    __device__ void get(float x[1]) const { x[0] = v; }
+    __device__ static void store(void* base, long long i, const float x[1])
+    {
+        if constexpr (std::is_same_v<T, F32>)
+            static_cast<float*>(base)[i] = x[0];
+        else if constexpr (std::is_same_v<T, F16>)
+            static_cast<_Float16*>(base)[i] = static_cast<_Float16>(x[0]);
+        else
+            static_cast<uint16_t*>(base)[i] = static_cast<uint16_t>(to_bf16_bits(x[0]));
+    }
+};
+template <typename T>
+struct Piece<T, 8>
+{
+    Raw8<T> r;
+    __device__ void load(const void* base, long long i) { ld_raw8<T>(base, i, r); }
+    __device__ void get(float x[8]) const { raw8_float(r, x); }
+    __device__ static void store(void* base, long long i, const float x[8]) { st8<T>(base, i, x); }
+};
+template <>
+struct Piece<F32, 4>
+{
+    float4 r;
+    __device__ void load(const void* base, long long i) { r = *reinterpret_cast<const float4*>(static_cast<const float*>(base) + i); }
+    __device__ void get(float x[4]) const
+    {
+        x[0] = r.x; x[1] = r.y; x[2] = r.z; x[3] = r.w;
+    }
+    __device__ static void store(void* base, long long i, const float x[4])
+    {
+        *reinterpret_cast<float4*>(static_cast<float*>(base) + i) = make_float4(x[0], x[1], x[2], x[3]);
+    }
+};
+
+// Elements of a 16-byte access.
+template <typename T>
+constexpr int wide()
+{
+    return 16 / elem_bytes<T>();
+}
+
+__device__ inline float wave_sum(float v)
+{
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1)
+        v += __shfl_xor(v, d, 64);
+    return v;
+}
+
+// Joins `entries` pieces (count n(e), mean, M2) whose counts add up to `total`,
+// one wave; every lane receives the result.
+template <typename N, typename M, typename S>
+__device__ inline void join(int entries, float total, int lane, N n, M mean, S m2, float* out_mean, float* out_m2)
+{
+    const float ref = mean(0);
+    float d = 0.f;
+    for (int e = lane; e < entries; e += 64)
+        d += n(e) * (mean(e) - ref);
+    const float mu = ref + wave_sum(d) / total;
+    float s = 0.f;
+    for (int e = lane; e < entries; e += 64)
+    {
+        const float off = mean(e) - mu;
+        s += m2(e) + n(e) * off * off;
+    }
+    *out_mean = mu;
+    *out_m2 = wave_sum(s);
+}
+
+// Rows of 0 .. rows - 1 that row lane r of `lanes` takes.
+__device__ inline int lane_rows(int rows, int lanes, int r)
+{
+    return r < rows ? (rows - 1 - r) / lanes + 1 : 0;
+}
+
+// gamma and beta of V channels, with the group's mean and 1 / sqrt(var + eps)
+// folded into the scale.
+template <int V>
+struct Affine
+{
+    float mean[V], a[V], b[V];
+    template <typename G>
+    __device__ void load(const NormArgs& p, int c0, G stat)
+    {
+#pragma unroll
+        for (int e = 0; e < V; e++)
+        {
+            const float2 s = stat(c0 + e);
+            mean[e] = s.x;
+            a[e] = s.y * (p.gamma ? p.gamma[c0 + e] : 1.f);
+            b[e] = p.beta ? p.beta[c0 + e] : 0.f;
+        }
+    }
+    template <int ACT, bool EXACT>
+    __device__ void apply(float x[V]) const
+    {
+#pragma unroll
+        for (int e = 0; e < V; e++)
+            x[e] = activate<ACT, EXACT>(__builtin_fmaf(x[e] - mean[e], a[e], b[e]));
+    }
+};
+
+// Slab form: workgroup (image, slab of slab_groups groups), at most KEEP rows
+// of V channels per thread.
+template <typename T, int V, int KEEP, int ACT>
+__global__ __launch_bounds__(kSlabThreads) void norm_slab_kernel(NormArgs p)
+{
+    extern __shared__ __attribute__((aligned(16))) float smem[];
+    const int image = blockIdx.x / p.slabs;
+    const int g0 = (blockIdx.x - image * p.slabs) * p.slab_groups;
+    const int ng = min(p.slab_groups, p.groups - g0);
+    const int c_base = g0 * p.width;
+    const int sc = ng * p.width;     // channels of this slab, a multiple of V
+    const int nc = sc / V;
+    const int lanes = blockDim.x / nc;
+    const int r0 = threadIdx.x / nc;
+    const int c = (threadIdx.x - r0 * nc) * V;
+    const bool active = r0 < lanes;
+    const int mine = active ? lane_rows(p.rows, lanes, r0) : 0;
+    const long long xi = image * p.x_image + c_base + c;
+
+    Piece<T, V> keep[KEEP];
+#pragma unroll
+    for (int k = 0; k < KEEP; k++)
+        if (k < mine)
+            keep[k].load(p.x, xi + static_cast<long long>(r0 + k * lanes) * p.x_row);
+    float mean[V], m2[V];
+#pragma unroll
+    for (int e = 0; e < V; e++)
+        mean[e] = m2[e] = 0.f;
+#pragma unroll
+    for (int k = 0; k < KEEP; k++)
+        if (k < mine)
+        {
+            float x[V];
+            keep[k].get(x);
+#pragma unroll
+            for (int e = 0; e < V; e++)
+                mean[e] += x[e];
+        }
+    const float inv = 1.f / static_cast<float>(max(mine, 1));
+#pragma unroll
+    for (int e = 0; e < V; e++)
+        mean[e] *= inv;
+#pragma unroll
+    for (int k = 0; k < KEEP; k++)
+        if (k < mine)
+        {
+            float x[V];
+            keep[k].get(x);
+#pragma unroll
+            for (int e = 0; e < V; e++)
+                m2[e] += (x[e] - mean[e]) * (x[e] - mean[e]);
+        }
+    float* s_mean = smem;
+    float* s_m2 = smem + lanes * sc;
+    float2* s_stat = reinterpret_cast<float2*>(smem + 2 * lanes * sc);
+    if (active)
+#pragma unroll
+        for (int e = 0; e < V; e++)
+        {
+            s_mean[r0 * sc + c + e] = mean[e];
+            s_m2[r0 * sc + c + e] = m2[e];
+        }
+    __syncthreads();
+    const int wave = threadIdx.x >> 6;
+    const int used = min(lanes, p.rows); // row lanes that hold a row
+    const float total = static_cast<float>(p.rows) * static_cast<float>(p.width);
+    for (int g = wave; g < ng; g += blockDim.x >> 6)
+    {
+        auto at = [&](int e) { const int r = e / p.width; return r * sc + g * p.width + (e - r * p.width); };
+        float mu, s;
+        join(used * p.width, total, threadIdx.x & 63,
+             [&](int e) { return static_cast<float>(lane_rows(p.rows, lanes, e / p.width)); },
+             [&](int e) { return s_mean[at(e)]; }, [&](int e) { return s_m2[at(e)]; }, &mu, &s);
+        if ((threadIdx.x & 63) == 0)
+            s_stat[g] = make_float2(mu, 1.f / sqrtf(s / total + p.eps));
+    }
+    __syncthreads();
+    if (!active)
+        return;
+    Affine<V> f;
+    {
+        NormArgs q = p;
+        q.gamma = p.gamma ? p.gamma + c_base : nullptr;
+        q.beta = p.beta ? p.beta + c_base : nullptr;
+        f.load(q, c, [&](int ch) { return s_stat[ch / p.width]; });
+    }
+    const long long yi = image * p.y_image + c_base + c;
+#pragma unroll
+    for (int k = 0; k < KEEP; k++)
+        if (k < mine)
+        {
+            float x[V];
+            keep[k].get(x);
+            f.template apply<ACT, std::is_same_v<T, F32>>(x);
+            Piece<T, V>::store(p.y, yi + static_cast<long long>(r0 + k * lanes) * p.y_row, x);
+        }
+}
+
+// Channels are taken by the 256 threads of a workgroup V at a time; where they
+// are more than 256 V, in rounds.
+struct Columns
+{
+    int nc, lanes, rounds;
+};
+template <int V>
+__host__ __device__ inline Columns columns(int channels)
+{
+    Columns k;
+    k.nc = channels / V;
+    k.lanes = k.nc >= kRowThreads ? 1 : kRowThreads / k.nc;
+    k.rounds = (k.nc + kRowThreads - 1) / kRowThreads;
+    return k;
+}
+
+// Rows form, first launch: workgroup (image, run of chunk_rows rows).
+template <typename T, int V>
+__global__ __launch_bounds__(kRowThreads) void norm_stats_kernel(NormArgs p)
+{
+    extern __shared__ __attribute__((aligned(16))) float smem[];
+    constexpr int kHeld = V == 1 ? 16 : 8; // rows in registers at a time
+    const int image = blockIdx.x / p.chunks;
+    const int chunk = blockIdx.x - image * p.chunks;
+    const int first = chunk * p.chunk_rows;
+    const int rows = min(p.chunk_rows, p.rows - first);
+    const Columns k = columns<V>(p.channels);
+    float* s_mean = smem;
+    float* s_m2 = smem + k.lanes * p.channels;
+    for (int round = 0; round < k.rounds; round++)
+    {
+        const int r0 = k.rounds > 1 ? 0 : threadIdx.x / k.nc;
+        const int col = k.rounds > 1 ? round * kRowThreads + threadIdx.x : threadIdx.x - r0 * k.nc;
+        if (r0 >= k.lanes || col >= k.nc)
+            continue;
+        const int mine = lane_rows(rows, k.lanes, r0);
+        long long at = image * p.x_image + static_cast<long long>(first + r0) * p.x_row + col * V;
+        const long long step = k.lanes * p.x_row;
+        float mean[V], m2[V];
+#pragma unroll
+        for (int e = 0; e < V; e++)
+            mean[e] = m2[e] = 0.f;
+        int done = 0;
+        for (; done + kHeld <= mine; done += kHeld)
+        {
+            Piece<T, V> h[kHeld];
+#pragma unroll
+            for (int i = 0; i < kHeld; i++)
+                h[i].load(p.x, at + i * step);
+            at += kHeld * step;
+            float bm[V], bs[V];
+#pragma unroll
+            for (int e = 0; e < V; e++)
+                bm[e] = bs[e] = 0.f;
+#pragma unroll
+            for (int i = 0; i < kHeld; i++)
+            {
+                float x[V];
+                h[i].get(x);
+#pragma unroll
+                for (int e = 0; e < V; e++)
+                    bm[e] += x[e];
+            }
+#pragma unroll
+            for (int e = 0; e < V; e++)
+                bm[e] *= 1.f / kHeld;
+#pragma unroll
+            for (int i = 0; i < kHeld; i++)
+            {
+                float x[V];
+                h[i].get(x);
+#pragma unroll
+                for (int e = 0; e < V; e++)
+                    bs[e] += (x[e] - bm[e]) * (x[e] - bm[e]);
+            }
+            const float share = static_cast<float>(kHeld) / static_cast<float>(done + kHeld);
+            const float both = share * static_cast<float>(done);
+#pragma unroll
+            for (int e = 0; e < V; e++)
+            {
+                const float d = bm[e] - mean[e];
+                mean[e] += d * share;
+                m2[e] += bs[e] + d * d * both;
+            }
+        }
+        for (; done < mine; done++)
+        {
+            Piece<T, V> h;
+            h.load(p.x, at);
+            at += step;
+            float x[V];
+            h.get(x);
+            const float share = 1.f / static_cast<float>(done + 1);
+#pragma unroll
+            for (int e = 0; e < V; e++)
+            {
+                const float d = x[e] - mean[e];
+                mean[e] += d * share;
+                m2[e] += d * (x[e] - mean[e]);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < V; e++)
+        {
+            s_mean[r0 * p.channels + col * V + e] = mean[e];
+            s_m2[r0 * p.channels + col * V + e] = m2[e];
+        }
+    }
+    __syncthreads();
+    const int used = min(k.lanes, rows);
+    const float total = static_cast<float>(rows) * static_cast<float>(p.width);
+    const int lane = threadIdx.x & 63;
+    for (int g = threadIdx.x >> 6; g < p.groups; g += kRowThreads >> 6)
+    {
+        auto at = [&](int e) { const int r = e / p.width; return r * p.channels + g * p.width + (e - r * p.width); };
+        float mu, s;
+        join(used * p.width, total, lane,
+             [&](int e) { return static_cast<float>(lane_rows(rows, k.lanes, e / p.width)); },
+             [&](int e) { return s_mean[at(e)]; }, [&](int e) { return s_m2[at(e)]; }, &mu, &s);
+        if (lane == 0)
+            p.part[(static_cast<long long>(image) * p.groups + g) * p.chunks + chunk] = make_float2(mu, s);
+    }
+}
+
+// Rows form, second launch: one wave per (image, group).
+__global__ __launch_bounds__(64) void norm_join_kernel(NormArgs p)
+{
+    const float2* part = p.part + static_cast<long long>(blockIdx.x) * p.chunks;
+    const float w = static_cast<float>(p.width);
+    const float total = static_cast<float>(p.rows) * w;
+    float mu, s;
+    join(p.chunks, total, threadIdx.x,
+         [&](int e) { return w * static_cast<float>(min(p.chunk_rows, p.rows - e * p.chunk_rows)); },
+         [&](int e) { return part[e].x; }, [&](int e) { return part[e].y; }, &mu, &s);
+    if (threadIdx.x == 0)
+        p.stat[blockIdx.x] = make_float2(mu, 1.f / sqrtf(s / total + p.eps));
+}
+
+// Rows form, third launch.
+template <typename T, int V, int ACT>
+__global__ __launch_bounds__(kRowThreads) void norm_apply_kernel(NormArgs p)
+{
+    constexpr int kHeld = V == 1 ? 16 : 8;
+    const int image = blockIdx.x / p.chunks;
+    const int first = (blockIdx.x - image * p.chunks) * p.chunk_rows;
+    const int rows = min(p.chunk_rows, p.rows - first);
+    const Columns k = columns<V>(p.channels);
+    const float2* stat = p.stat + static_cast<long long>(image) * p.groups;
+    for (int round = 0; round < k.rounds; round++)
+    {
+        const int r0 = k.rounds > 1 ? 0 : threadIdx.x / k.nc;
+        const int col = k.rounds > 1 ? round * kRowThreads + threadIdx.x : threadIdx.x - r0 * k.nc;
+        if (r0 >= k.lanes || col >= k.nc)
+            continue;
+        Affine<V> f;
+        f.load(p, col * V, [&](int ch) { return stat[ch / p.width]; });
+        const int mine = lane_rows(rows, k.lanes, r0);
+        long long xi = image * p.x_image + static_cast<long long>(first + r0) * p.x_row + col * V;
+        long long yi = image * p.y_image + static_cast<long long>(first + r0) * p.y_row + col * V;
+        const long long xs = k.lanes * p.x_row;
+        const long long ys = k.lanes * p.y_row;
+        for (int done = 0; done < mine; done += kHeld)
+        {
+            Piece<T, V> h[kHeld];
+#pragma unroll
+            for (int i = 0; i < kHeld; i++)
+                if (done + i < mine)
+                    h[i].load(p.x, xi + i * xs);
+#pragma unroll
+            for (int i = 0; i < kHeld; i++)
+                if (done + i < mine)
+                {
+                    float x[V];
+                    h[i].get(x);
+                    f.template apply<ACT, std::is_same_v<T, F32>>(x);
+                    Piece<T, V>::store(p.y, yi + i * ys, x);
+                }
+            xi += kHeld * xs;
+            yi += kHeld * ys;
+        }
+    }
+}
+
+// The rows form's runs: enough workgroups for 256 CUs, at least 64 KB each.
+void plan_rows(NormArgs* p, int images, int bytes)
+{
+    const long long row_bytes = static_cast<long long>(p->channels) * bytes;
+    const long long want = (static_cast<long long>(images) * p->rows + 1023) / 1024;
+    const long long least = std::max(1LL, 65536 / row_bytes);
+    p->chunk_rows = static_cast<int>(std::min<long long>(p->rows, std::max(want, least)));
+    p->chunks = (p->rows + p->chunk_rows - 1) / p->chunk_rows;
+}
+
+// Bytes of (mean, M2) of every run and (mean, rstd) of every group.
+long long rows_workspace(const NormArgs& p, int images)
+{
+    return static_cast<long long>(images) * p.groups * (p.chunks + 1) * static_cast<long long>(sizeof(float2));
+}
+
+// The slab form's shape for pieces of V elements, or threads = 0 where an
+// image does not fit: whole groups whose channels are a multiple of V, 64
+// bytes of a row at least (a quarter of the groups otherwise share a line).
+struct Slab
+{
+    int groups, threads, lds;
+};
+Slab plan_slab(const NormArgs& p, int v, int keep, int bytes)
+{
+    int g = 1;
+    while (g < p.groups && (g * p.width % v != 0 || g * p.width * bytes < 64))
+        g++;
+    const int sc = g * p.width;
+    const int nc = sc / v;
+    if (sc % v != 0 || nc > kSlabThreads)
+        return Slab{0, 0, 0};
+    // the fewest threads that hold the rows in half of the registers, or all
+    // of them
+    for (int threads : {256, 512, 1024})
+    {
+        const int lanes = threads / nc;
+        if (lanes > 0 && p.rows <= lanes * (threads < 1024 ? keep / 2 : keep))
+            // the last slab may be narrower and have more row lanes
+            return Slab{g, threads, 2 * threads * v * 4 + g * 8};
+    }
+    return Slab{0, 0, 0};
+}
+
+constexpr int kKeepWide = 8;
+constexpr int kKeepOne = 32;
+
+template <typename T, int V, int ACT>
+int run_norm(NormArgs p, int images, bool slab, const Slab& s, hipStream_t stream)
+{
+    if (slab)
+    {
+        constexpr int kKeep = V == 1 ? kKeepOne : kKeepWide;
+        p.slab_groups = s.groups;
+        p.slabs = (p.groups + s.groups - 1) / s.groups;
+        const long long grid = static_cast<long long>(images) * p.slabs;
+        if (grid > INT_MAX)
+            return set_error(SV2_EUNSUPPORTED, "sv2_group_norm: too many images");
+        const void* fn = reinterpret_cast<const void*>(&norm_slab_kernel<T, V, kKeep, ACT>);
+        const int rc = set_dynamic_lds(fn, s.lds, "norm_slab: dynamic LDS attribute");
+        if (rc != SV2_OK)
+            return rc;
+        hipLaunchKernelGGL((norm_slab_kernel<T, V, kKeep, ACT>), dim3(static_cast<unsigned>(grid)), dim3(s.threads),
+                           s.lds, stream, p);
+    }
+    else
+    {
+        const long long grid = static_cast<long long>(images) * p.chunks;
+        const long long joins = static_cast<long long>(images) * p.groups;
+        if (grid > INT_MAX || joins > INT_MAX)
+            return set_error(SV2_EUNSUPPORTED, "sv2_group_norm: too many images");
+        const int lds = 2 * columns<V>(p.channels).lanes * p.channels * 4;
+        const void* fn = reinterpret_cast<const void*>(&norm_stats_kernel<T, V>);
+        const int rc = set_dynamic_lds(fn, lds, "norm_stats: dynamic LDS attribute");
+        if (rc != SV2_OK)
+            return rc;
+        hipLaunchKernelGGL((norm_stats_kernel<T, V>), dim3(static_cast<unsigned>(grid)), dim3(kRowThreads), lds, stream, p);
+        hipLaunchKernelGGL(norm_join_kernel, dim3(static_cast<unsigned>(joins)), dim3(64), 0, stream, p);
+        hipLaunchKernelGGL((norm_apply_kernel<T, V, ACT>), dim3(static_cast<unsigned>(grid)), dim3(kRowThreads), 0, stream, p);
+    }
+    const hipError_t err = hipGetLastError();
+    return err == hipSuccess ? SV2_OK : hip_error(err, "sv2_group_norm launch");
+}
+
+template <typename T, int V>
+int run_act(const NormArgs& p, int images, int activation, bool slab, const Slab& s, hipStream_t stream)
+{
+    switch (activation)
+    {
+    case SV2_ACT_SILU: return run_norm<T, V, SV2_ACT_SILU>(p, images, slab, s, stream);
+    case SV2_ACT_GELU: return run_norm<T, V, SV2_ACT_GELU>(p, images, slab, s, stream);
+    case SV2_ACT_GELU_TANH: return run_norm<T, V, SV2_ACT_GELU_TANH>(p, images, slab, s, stream);
+    default: return run_norm<T, V, SV2_ACT_NONE>(p, images, slab, s, stream);
+    }
+}
+
+int check_sizes(int dtype, int images, int rows, int channels, int groups, const char* what)
+{
+    if ((dtype != SV2_F32 && dtype != SV2_F16 && dtype != SV2_BF16) || images < 0 || rows < 0 || channels <= 0 ||
+        groups <= 0 || channels % groups != 0)
+        return set_error(SV2_EINVAL, std::string(what) + ": bad type or sizes (channels must be a multiple of groups)");
+    if (channels > kMaxChannels)
+        return set_error(SV2_EUNSUPPORTED, std::string(what) + ": more than 8192 channels");
+    return SV2_OK;
+}
+
+} // namespace
+} // namespace sv2
+
+extern "C" int64_t sv2_group_norm_workspace(int dtype, int images, int rows, int channels, int groups)
+try
+{
+    using namespace sv2;
+    const int rc = check_sizes(dtype, images, rows, channels, groups, "sv2_group_norm_workspace");
+    if (rc != SV2_OK)
+        return rc;
+    if (images == 0 || rows == 0)
+        return 0;
+    NormArgs p{};
+    p.rows = rows;
+    p.channels = channels;
+    p.groups = groups;
+    p.width = channels / groups;
+    const int bytes = dtype == SV2_F32 ? 4 : 2;
+    // where even single elements fit the slab form, every layout does
+    if (plan_slab(p, 1, kKeepOne, bytes).threads > 0 && plan_slab(p, 16 / bytes, kKeepWide, bytes).threads > 0)
+        return 0;
+    plan_rows(&p, images, bytes);
+    return rows_workspace(p, images);
+}
+catch (...)
+{
+    return sv2::caught_exception("sv2_group_norm_workspace");
+}
+
+extern "C" int sv2_group_norm(const void* x, int64_t x_image_stride, int64_t x_row_stride, void* y,
+                              int64_t y_image_stride, int64_t y_row_stride, int dtype, int images, int rows,
+                              int channels, int groups, float eps, const float* gamma, const float* beta,
+                              int activation, void* workspace, size_t workspace_bytes, void* stream)
+try
+{
+    using namespace sv2;
+    const int rc = check_sizes(dtype, images, rows, channels, groups, "sv2_group_norm");
+    if (rc != SV2_OK)
+        return rc;
+    if (activation < SV2_ACT_NONE || activation > SV2_ACT_GELU_TANH || !(eps >= 0.f))
+        return set_error(SV2_EINVAL, "sv2_group_norm: unknown activation or negative eps");
+    if (images == 0 || rows == 0)
+        return SV2_OK;
+    const int bytes = dtype == SV2_F32 ? 4 : 2;
+    if (!x || !y)
+        return set_error(SV2_EINVAL, "sv2_group_norm: null pointer");
+    if (misaligned(x, bytes) || misaligned(y, bytes) || misaligned(gamma, 4) || misaligned(beta, 4) ||
+        misaligned(workspace, 8))
+        return set_error(SV2_EINVAL, "sv2_group_norm: a pointer is not aligned to its elements");
+    if (x_row_stride < channels || y_row_stride < channels ||
+        (images > 1 && (x_image_stride < 0 || y_image_stride < channels)))
+        return set_error(SV2_EINVAL, "sv2_group_norm: a stride below the channel count");
+    NormArgs p{};
+    p.x = x;
+    p.y = y;
+    p.x_image = x_image_stride;
+    p.x_row = x_row_stride;
+    p.y_image = y_image_stride;
+    p.y_row = y_row_stride;
+    p.gamma = gamma;
+    p.beta = beta;
+    p.rows = rows;
+    p.channels = channels;
+    p.groups = groups;
+    p.width = channels / groups;
+    p.eps = eps;
+    const int v = 16 / bytes;
+    const bool one_image = images == 1; // its image strides are not read
+    const bool wide = channels % v == 0 && x_row_stride % v == 0 && y_row_stride % v == 0 && !misaligned(x, 16) &&
+                      !misaligned(y, 16) && (one_image || (x_image_stride % v == 0 && y_image_stride % v == 0));
+    const Slab s = plan_slab(p, wide ? v : 1, wide ? kKeepWide : kKeepOne, bytes);
+    const bool slab = s.threads > 0;
+    if (!slab)
+    {
+        plan_rows(&p, images, bytes);
+        if (!workspace || workspace_bytes < static_cast<size_t>(rows_workspace(p, images)))
+            return set_error(SV2_EINVAL, "sv2_group_norm: workspace missing or too small");
+        p.part = static_cast<float2*>(workspace);
+        p.stat = p.part + static_cast<long long>(images) * groups * p.chunks;
+    }
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    if (dtype == SV2_F32)
+        return wide ? run_act<vec::F32, 4>(p, images, activation, slab, s, st)
+                    : run_act<vec::F32, 1>(p, images, activation, slab, s, st);
+    if (dtype == SV2_F16)
+        return wide ? run_act<vec::F16, 8>(p, images, activation, slab, s, st)
+                    : run_act<vec::F16, 1>(p, images, activation, slab, s, st);
+    return wide ? run_act<vec::BF16, 8>(p, images, activation, slab, s, st)
+                : run_act<vec::BF16, 1>(p, images, activation, slab, s, st);
+}
+catch (...)
+{
+    return sv2::caught_exception("sv2_group_norm");
+}

@@ -1,0 +1,291 @@
+// Matrix product with bias, activation and residual in its epilogue:
+//
+//   y[m][n] = act(sum_k x[m][k] w[n][k] + bias[n]) + residual[m][n]
+//
+// fp16 or bf16 operands, fp32 sums, one rounding at the end.  Any sizes, row
+// strides and element alignment.
+#include "sv2_internal.h"
+#include "activation.h"
+#include "vec_io.h"
+
+#include <algorithm>
+#include <climits>
+
+namespace sv2
+{
+namespace
+{
+
+typedef __attribute__((ext_vector_type(8))) _Float16 h8;
+typedef __attribute__((ext_vector_type(8))) __bf16 b8;
+typedef __attribute__((ext_vector_type(4))) float f4;
+typedef __attribute__((ext_vector_type(4))) unsigned u4;
+typedef __attribute__((ext_vector_type(2))) unsigned u2;
+typedef __attribute__((ext_vector_type(4), aligned(2))) unsigned u4u; // 16 bytes at any element
+
+struct HalfIO
+{
+    static __device__ f4 mfma(u4 a, u4 b, f4 c)
+    {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+    }
+    static __device__ float to_float(uint16_t v) { return static_cast<float>(__builtin_bit_cast(_Float16, v)); }
+    static __device__ uint16_t from_float(float v) { return __builtin_bit_cast(uint16_t, static_cast<_Float16>(v)); }
+};
+struct BfloatIO
+{
+    static __device__ f4 mfma(u4 a, u4 b, f4 c)
+    {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+    }
+    static __device__ float to_float(uint16_t v) { return __builtin_bit_cast(float, static_cast<uint32_t>(v) << 16); }
+    static __device__ uint16_t from_float(float v) { return __builtin_bit_cast(uint16_t, static_cast<__bf16>(v)); }
+};
+
+struct LinearParams
+{
+    const uint16_t* x;
+    const uint16_t* w;
+    uint16_t* y;
+    const uint16_t* r;
+    const float* bias;
+    long long ldx, ldw, ldy, ldr;
+    int m, n, k;
+    int tiles_m, tiles_n;
+    int vec4; // rows of y and the residual hold whole aligned groups of 4
+};
+
+constexpr int kTile = 128;
+constexpr int kBK = 32;
+constexpr int kPitch = kBK * 2 + 16; // bytes of an LDS row: 16 rows of one chunk start in different banks
+
+// 8 elements of a row from column k on, zeros past `k_end`.
+__device__ inline u4 load8(const uint16_t* row, int k, int k_end)
+{
+    if (k + 8 <= k_end)
+        return *reinterpret_cast<const u4u*>(row + k);
+    u4 v = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+        if (k + e < k_end)
+            v[e >> 1] |= static_cast<unsigned>(row[k + e]) << (16 * (e & 1));
+    return v;
+}
+
+// Four columns of one output row.
+template <typename IO, int ACT>
+__device__ inline void finish4(const LinearParams& p, int m, int n, f4 v)
+{
+    if (m >= p.m || n >= p.n)
+        return;
+    uint16_t* y = p.y + m * p.ldy + n;
+    const uint16_t* r = p.r ? p.r + m * p.ldr + n : nullptr;
+    if (p.vec4)
+    {
+        u2 old = {0u, 0u};
+        if (r)
+            old = *reinterpret_cast<const u2*>(r);
+        uint16_t o[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+        {
+            float t = v[e];
+            if (p.bias)
+                t += p.bias[n + e];
+            t = activate<ACT, false>(t);
+            if (r)
+                t += IO::to_float(static_cast<uint16_t>(old[e >> 1] >> (16 * (e & 1))));
+            o[e] = IO::from_float(t);
+        }
+        *reinterpret_cast<u2*>(y) = u2{o[0] | static_cast<unsigned>(o[1]) << 16, o[2] | static_cast<unsigned>(o[3]) << 16};
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        if (n + e < p.n)
+        {
+            float t = v[e];
+            if (p.bias)
+                t += p.bias[n + e];
+            t = activate<ACT, false>(t);
+            if (r)
+                t += IO::to_float(r[e]);
+            y[e] = IO::from_float(t);
+        }
+}
+
+// 128 x 128 outputs by 4 waves of 64 x 64, K in steps of 32 through registers
+// into two LDS buffers; the product is computed transposed (w as the first
+// operand), so a lane holds four columns of one output row.
+template <typename IO, int ACT>
+__global__ __launch_bounds__(256, 2) void linear_any_kernel(LinearParams p)
+{
+    __shared__ __attribute__((aligned(16))) char smem[2][2][kTile * kPitch];
+    const int tn = blockIdx.x % p.tiles_n;
+    const int tm = blockIdx.x / p.tiles_n;
+    const int m0 = tm * kTile;
+    const int n0 = tn * kTile;
+    const int lane = threadIdx.x & 63;
+    const int wave = threadIdx.x >> 6;
+    const int lr = lane & 15;
+    const int lq = lane >> 4;
+    const int wn = 64 * (wave & 1);
+    const int wm = 64 * (wave >> 1);
+
+    // this thread's chunks: rows threadIdx / 4 and + 64, chunk threadIdx % 4
+    const int cr = threadIdx.x >> 2;
+    const int cc = threadIdx.x & 3;
+    const uint16_t* xr[2];
+    const uint16_t* wr[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+    {
+        // rows past the end repeat the last one; their sums are not stored
+        xr[i] = p.x + min(m0 + cr + 64 * i, p.m - 1) * p.ldx;
+        wr[i] = p.w + min(n0 + cr + 64 * i, p.n - 1) * p.ldw;
+    }
+    u4 xv[2], wv[2];
+    auto load = [&](int k0) {
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+        {
+            xv[i] = load8(xr[i], k0 + 8 * cc, p.k);
+            wv[i] = load8(wr[i], k0 + 8 * cc, p.k);
+        }
+    };
+    auto put = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+        {
+            *reinterpret_cast<u4*>(&smem[buf][0][(cr + 64 * i) * kPitch + 16 * cc]) = wv[i];
+            *reinterpret_cast<u4*>(&smem[buf][1][(cr + 64 * i) * kPitch + 16 * cc]) = xv[i];
+        }
+    };
+    f4 acc[4][4];
+#pragma unroll
+    for (int t = 0; t < 4; t++)
+#pragma unroll
+        for (int b = 0; b < 4; b++)
+            acc[t][b] = f4{0.f, 0.f, 0.f, 0.f};
+    load(0);
+    put(0);
+    __syncthreads();
+    const int steps = (p.k + kBK - 1) / kBK;
+    for (int s = 0; s < steps; s++)
+    {
+        const int buf = s & 1;
+        if (s + 1 < steps)
+            load((s + 1) * kBK);
+        u4 a[4], b[4];
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+        {
+            a[t] = *reinterpret_cast<const u4*>(&smem[buf][0][(wn + 16 * t + lr) * kPitch + 16 * lq]);
+            b[t] = *reinterpret_cast<const u4*>(&smem[buf][1][(wm + 16 * t + lr) * kPitch + 16 * lq]);
+        }
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+                acc[t][u] = IO::mfma(a[t], b[u], acc[t][u]);
+        if (s + 1 < steps)
+            put(buf ^ 1);
+        __syncthreads();
+    }
+#pragma unroll
+    for (int t = 0; t < 4; t++)
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+            finish4<IO, ACT>(p, m0 + wm + 16 * u + lr, n0 + wn + 16 * t + 4 * lq, acc[t][u]);
+}
+
+template <typename IO, int ACT>
+int run_linear(LinearParams p, hipStream_t stream)
+{
+    p.tiles_m = (p.m + kTile - 1) / kTile;
+    p.tiles_n = (p.n + kTile - 1) / kTile;
+    const long long total = static_cast<long long>(p.tiles_m) * p.tiles_n;
+    if (total > INT_MAX)
+        return set_error(SV2_EUNSUPPORTED, "sv2_linear: too many tiles");
+    hipLaunchKernelGGL((linear_any_kernel<IO, ACT>), dim3(static_cast<unsigned>(total)), dim3(256), 0, stream, p);
+    const hipError_t err = hipGetLastError();
+    return err == hipSuccess ? SV2_OK : hip_error(err, "sv2_linear launch");
+}
+
+template <typename IO>
+int run_act(const LinearParams& p, int activation, hipStream_t stream)
+{
+    switch (activation)
+    {
+    case SV2_ACT_SILU: return run_linear<IO, SV2_ACT_SILU>(p, stream);
+    case SV2_ACT_GELU: return run_linear<IO, SV2_ACT_GELU>(p, stream);
+    case SV2_ACT_GELU_TANH: return run_linear<IO, SV2_ACT_GELU_TANH>(p, stream);
+    default: return run_linear<IO, SV2_ACT_NONE>(p, stream);
+    }
+}
+
+int check_linear(const sv2_linear_args* a, const char* what)
+{
+    auto bad = [&](const char* why) { return set_error(SV2_EINVAL, std::string(what) + ": " + why); };
+    if (!a)
+        return bad("null arguments");
+    if (a->rows < 0 || a->in <= 0 || a->out < 0)
+        return bad("negative sizes");
+    if (a->dtype != SV2_F16 && a->dtype != SV2_BF16)
+        return set_error(a->dtype == SV2_F32 ? SV2_EUNSUPPORTED : SV2_EINVAL, std::string(what) + ": dtype must be SV2_F16 or SV2_BF16");
+    if (a->activation < SV2_ACT_NONE || a->activation > SV2_ACT_GELU_TANH)
+        return bad("unknown activation");
+    if (a->x_stride < a->in || a->w_stride < a->in || a->y_stride < a->out || (a->residual && a->residual_stride < a->out))
+        return bad("a row stride below the row's length");
+    return SV2_OK;
+}
+
+} // namespace
+} // namespace sv2
+
+extern "C" int64_t sv2_linear_workspace(const sv2_linear_args* args)
+try
+{
+    const int rc = sv2::check_linear(args, "sv2_linear_workspace");
+    return rc != SV2_OK ? rc : 0;
+}
+catch (...)
+{
+    return sv2::caught_exception("sv2_linear_workspace");
+}
+
+extern "C" int sv2_linear(const sv2_linear_args* args, void* stream)
+try
+{
+    using namespace sv2;
+    const int rc = check_linear(args, "sv2_linear");
+    if (rc != SV2_OK)
+        return rc;
+    const sv2_linear_args& a = *args;
+    if (a.rows == 0 || a.out == 0)
+        return SV2_OK;
+    if (!a.x || !a.w || !a.y)
+        return set_error(SV2_EINVAL, "sv2_linear: null pointer");
+    if (misaligned(a.x, 2) || misaligned(a.w, 2) || misaligned(a.y, 2) || misaligned(a.residual, 2) || misaligned(a.bias, 4))
+        return set_error(SV2_EINVAL, "sv2_linear: a pointer is not aligned to its elements");
+    LinearParams p{};
+    p.x = static_cast<const uint16_t*>(a.x);
+    p.w = static_cast<const uint16_t*>(a.w);
+    p.y = static_cast<uint16_t*>(a.y);
+    p.r = static_cast<const uint16_t*>(a.residual);
+    p.bias = a.bias;
+    p.ldx = a.x_stride;
+    p.ldw = a.w_stride;
+    p.ldy = a.y_stride;
+    p.ldr = a.residual ? a.residual_stride : 0;
+    p.m = a.rows;
+    p.n = a.out;
+    p.k = a.in;
+    p.vec4 = p.n % 4 == 0 && p.ldy % 4 == 0 && p.ldr % 4 == 0 && !misaligned(p.y, 8) && !misaligned(p.r, 8);
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    return a.dtype == SV2_F16 ? run_act<HalfIO>(p, a.activation, st) : run_act<BfloatIO>(p, a.activation, st);
+}
+catch (...)
+{
+    return sv2::caught_exception("sv2_linear");
+}

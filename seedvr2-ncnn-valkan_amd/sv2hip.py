@@ -23,6 +23,7 @@ SV2_EDEVICE = -100
 F32, F16, BF16 = 0, 1, 2
 ROPE_REFERENCE, ROPE_ABSOLUTE, ROPE_NONE = 0, 1, 2
 VERIFY_NONE, VERIFY_IF_PRESENT, VERIFY_STRICT = 0, 1, 2
+ACT_NONE, ACT_SILU, ACT_GELU, ACT_GELU_TANH = 0, 1, 2, 3
 STAGE_TEXT_PREPARE, STAGE_WINDOWS, STAGE_TEXT_REDUCE, STAGE_ALL = 1, 2, 4, 7
 
 # Exported symbols declared in include/seedvr2_hip.h.
@@ -81,6 +82,12 @@ EXPORTS = [
     "sv2_inner_product_f16_few_workspace",
     "sv2_inner_product_f16_few",
     "sv2_inner_product_f32",
+    "sv2_sliding_attention_workspace",
+    "sv2_sliding_attention",
+    "sv2_group_norm_workspace",
+    "sv2_group_norm",
+    "sv2_linear_workspace",
+    "sv2_linear",
     "sv2_euler_timesteps",
     "sv2_condition_ratio",
     "sv2_make_condition",
@@ -135,6 +142,39 @@ class AttnArgs(ctypes.Structure):
         ("workspace_bytes", ctypes.c_size_t),
         ("debug_pre", ctypes.c_void_p),
         ("exact", ctypes.c_int),
+    ]
+
+
+class SlidingAttnArgs(ctypes.Structure):
+    _fields_ = (
+        [(n, ctypes.c_int) for n in ("batch", "q_len", "kv_len", "heads", "kv_heads", "head_dim", "dtype", "left",
+                                     "right", "sinks")]
+        + [("scale", ctypes.c_float)]
+        + [(n, t) for x in ("q", "k", "v", "out") for n, t in (
+            (x, ctypes.c_void_p), (x + "_batch_stride", ctypes.c_int64), (x + "_token_stride", ctypes.c_int64),
+            (x + "_head_stride", ctypes.c_int64))]
+        + [("q_lens", ctypes.c_void_p), ("kv_lens", ctypes.c_void_p), ("lse", ctypes.c_void_p),
+           ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)])
+
+
+class LinearArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_int),
+        ("in_", ctypes.c_int),
+        ("out", ctypes.c_int),
+        ("dtype", ctypes.c_int),
+        ("activation", ctypes.c_int),
+        ("x", ctypes.c_void_p),
+        ("x_stride", ctypes.c_int64),
+        ("w", ctypes.c_void_p),
+        ("w_stride", ctypes.c_int64),
+        ("bias", ctypes.c_void_p),
+        ("residual", ctypes.c_void_p),
+        ("residual_stride", ctypes.c_int64),
+        ("y", ctypes.c_void_p),
+        ("y_stride", ctypes.c_int64),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
     ]
 
 
@@ -339,6 +379,20 @@ def load() -> ctypes.CDLL:
     lib.sv2_inner_product_f32.argtypes = [vp, vp, vp, vp, i, i, i, vp]
     lib.sv2_inner_product_f32.restype = i
     i64 = ctypes.c_int64
+    lib.sv2_sliding_attention_workspace.argtypes = [ctypes.POINTER(SlidingAttnArgs)]
+    lib.sv2_sliding_attention_workspace.restype = ctypes.c_int64
+    lib.sv2_sliding_attention.argtypes = [ctypes.POINTER(SlidingAttnArgs), vp]
+    lib.sv2_sliding_attention.restype = i
+    lib.sv2_group_norm_workspace.argtypes = [i, i, i, i, i]
+    lib.sv2_group_norm_workspace.restype = ctypes.c_int64
+    i64 = ctypes.c_int64
+    lib.sv2_group_norm.argtypes = [vp, i64, i64, vp, i64, i64, i, i, i, i, i, ctypes.c_float, vp, vp, i, vp,
+                                   ctypes.c_size_t, vp]
+    lib.sv2_group_norm.restype = i
+    lib.sv2_linear_workspace.argtypes = [ctypes.POINTER(LinearArgs)]
+    lib.sv2_linear_workspace.restype = ctypes.c_int64
+    lib.sv2_linear.argtypes = [ctypes.POINTER(LinearArgs), vp]
+    lib.sv2_linear.restype = i
     lib.sv2_euler_timesteps.argtypes = [i, vp]
     lib.sv2_euler_timesteps.restype = i
     lib.sv2_condition_ratio.argtypes = [c_f, i, i, i]
@@ -1103,6 +1157,130 @@ def inner_product_f16_few(x, w, y, epilogue=EPI_STORE, w_value=None, bias=None, 
           "sv2_inner_product_f16_few")
     return y
 
+
+
+def _need(name, t, dtype, shape, device):
+    """A device tensor of this type, shape and device whose last dimension is
+    contiguous."""
+    if not (t.is_cuda and t.dtype == dtype and tuple(t.shape) == shape and t.device == device
+            and (shape[-1] <= 1 or t.stride(-1) == 1)):
+        raise ValueError(f"{name} must be a {dtype} tensor {shape} on {device} with a contiguous last dimension")
+
+
+def _need_dense(name, t, dtype, shape, device):
+    if t is not None and not (t.is_cuda and t.dtype == dtype and tuple(t.shape) == shape and t.device == device
+                              and t.is_contiguous()):
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor {shape} on {device}")
+
+
+def _bound_workspace(workspace, need, like):
+    """`workspace`, or a new one where a call needs one and has none; its size
+    in bytes."""
+    import torch
+    if workspace is None:
+        if need == 0:
+            return None, 0
+        workspace = torch.empty(need, dtype=torch.uint8, device=like.device)
+    elif not (workspace.is_cuda and workspace.device == like.device and workspace.is_contiguous()):
+        raise ValueError(f"workspace must be a contiguous tensor on {like.device}")
+    return workspace, workspace.numel() * workspace.element_size()
+
+
+def _on(t):
+    """The device of `t` made current for a call."""
+    import torch
+    return torch.cuda.device(t.device)
+
+
+def _steps(t):
+    """Strides of all but the last dimension; 0 where there is nothing to step
+    over."""
+    return [s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape[:-1])]
+
+
+def sliding_attention(q, k, v, out, *, left, right=0, sinks=0, scale=None, q_lens=None, kv_lens=None, lse=None,
+                      workspace=None, stream=None):
+    """Attention of q [batch, q_len, heads, dim] over a cache k, v [batch,
+    kv_len, kv_heads, dim] with a sliding window and first tokens that stay
+    visible (sv2_sliding_attention), into `out` (as q) and `lse` [batch, heads,
+    q_len] fp32 when given.  The query of token i of a sequence stands at p =
+    kv_len - q_len + i and sees the keys j <= p + right with j < sinks or j >=
+    p - left; `q_lens`, `kv_lens`: int32 device tensors [batch] of each
+    sequence's own lengths.  `scale`: dim ** -0.5 when None.  Tensors may be
+    strided views with a contiguous last dimension."""
+    import torch
+    b, nq, h, d = q.shape
+    nk, g = k.shape[1], k.shape[2]
+    dev = q.device
+    for name, t, shape in (("q", q, (b, nq, h, d)), ("k", k, (b, nk, g, d)), ("v", v, (b, nk, g, d)),
+                           ("out", out, (b, nq, h, d))):
+        _need(name, t, q.dtype, shape, dev)
+    _need_dense("q_lens", q_lens, torch.int32, (b,), dev)
+    _need_dense("kv_lens", kv_lens, torch.int32, (b,), dev)
+    _need_dense("lse", lse, torch.float32, (b, h, nq), dev)
+    a = SlidingAttnArgs(b, nq, nk, h, g, d, torch_dtype_code(q), min(left, 2**31 - 1), min(right, 2**31 - 1), sinks,
+                        d ** -0.5 if scale is None else scale,
+                        q.data_ptr(), *_steps(q), k.data_ptr(), *_steps(k), v.data_ptr(), *_steps(v),
+                        out.data_ptr(), *_steps(out), None if q_lens is None else q_lens.data_ptr(),
+                        None if kv_lens is None else kv_lens.data_ptr(), None if lse is None else lse.data_ptr())
+    lib = load()
+    ref = ctypes.byref(a)
+    need = check(lib.sv2_sliding_attention_workspace(ref), "sv2_sliding_attention_workspace")
+    with _on(q):
+        workspace, a.workspace_bytes = _bound_workspace(workspace, need, q)
+        a.workspace = None if workspace is None else workspace.data_ptr()
+        check(lib.sv2_sliding_attention(ref, _stream(stream)), "sv2_sliding_attention")
+    return out
+
+
+def group_norm(x, y, groups, *, gamma=None, beta=None, eps=1e-5, activation=ACT_NONE, workspace=None, stream=None):
+    """y = act(group_norm(x) * gamma + beta) of a channels-last x [images, rows,
+    channels], per image and group (sv2_group_norm).  gamma, beta: fp32
+    [channels] or None; y may be x."""
+    import torch
+    n, rows, c = x.shape
+    _need("x", x, x.dtype, (n, rows, c), x.device)
+    _need("y", y, x.dtype, (n, rows, c), x.device)
+    _need_dense("gamma", gamma, torch.float32, (c,), x.device)
+    _need_dense("beta", beta, torch.float32, (c,), x.device)
+    lib = load()
+    code = torch_dtype_code(x)
+    need = check(lib.sv2_group_norm_workspace(code, n, rows, c, groups), "sv2_group_norm_workspace")
+    with _on(x):
+        workspace, size = _bound_workspace(workspace, need, x)
+        check(lib.sv2_group_norm(_ptr(x), x.stride(0), x.stride(1) if rows > 1 else c, _ptr(y), y.stride(0),
+                                 y.stride(1) if rows > 1 else c, code, n, rows, c, groups, eps, _ptr(gamma),
+                                 _ptr(beta), activation, _ptr(workspace), size, _stream(stream)), "sv2_group_norm")
+    return y
+
+
+def linear(x, w, y, *, bias=None, activation=ACT_NONE, residual=None, workspace=None, stream=None):
+    """y = act(x W^T + bias) + residual (sv2_linear): x [rows, in], w [out, in],
+    y and residual [rows, out], all fp16 or all bf16 with contiguous rows; bias
+    fp32 [out].  y may be the residual."""
+    import torch
+    rows, k = x.shape
+    n = w.shape[0]
+    for name, t, shape in (("x", x, (rows, k)), ("w", w, (n, k)), ("y", y, (rows, n))):
+        _need(name, t, x.dtype, shape, x.device)
+    _need_dense("bias", bias, torch.float32, (n,), x.device)
+    if residual is not None:
+        _need("residual", residual, x.dtype, (rows, n), x.device)
+
+    def step(t):
+        return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+    a = LinearArgs(rows, k, n, torch_dtype_code(x), activation, x.data_ptr(), step(x), w.data_ptr(), step(w),
+                   None if bias is None else bias.data_ptr(), None if residual is None else residual.data_ptr(),
+                   0 if residual is None else step(residual), y.data_ptr(), step(y))
+    lib = load()
+    ref = ctypes.byref(a)
+    need = check(lib.sv2_linear_workspace(ref), "sv2_linear_workspace")
+    with _on(x):
+        workspace, a.workspace_bytes = _bound_workspace(workspace, need, x)
+        a.workspace = None if workspace is None else workspace.data_ptr()
+        check(lib.sv2_linear(ref, _stream(stream)), "sv2_linear")
+    return y
 
 
 def sha256(data) -> bytes:
