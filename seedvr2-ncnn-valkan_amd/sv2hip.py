@@ -1160,42 +1160,71 @@ def inner_product_f16_few(x, w, y, epilogue=EPI_STORE, w_value=None, bias=None, 
 
 
 def _need(name, t, dtype, shape, device):
-    """A device tensor of this type, shape and device whose last dimension is
+    """A tensor of this type, shape and device whose last dimension is
     contiguous."""
-    if not (t.is_cuda and t.dtype == dtype and tuple(t.shape) == shape and t.device == device
-            and (shape[-1] <= 1 or t.stride(-1) == 1)):
-        raise ValueError(f"{name} must be a {dtype} tensor {shape} on {device} with a contiguous last dimension")
+    if t.dtype != dtype or t.shape != shape or t.device != device or (shape[-1] > 1 and t.stride(-1) != 1):
+        raise ValueError(f"{name} must be a {dtype} tensor {tuple(shape)} on {device} with a contiguous last dimension")
 
 
-def _need_dense(name, t, dtype, shape, device):
-    if t is not None and not (t.is_cuda and t.dtype == dtype and tuple(t.shape) == shape and t.device == device
-                              and t.is_contiguous()):
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor {shape} on {device}")
-
-
-def _bound_workspace(workspace, need, like):
-    """`workspace`, or a new one where a call needs one and has none; its size
-    in bytes."""
-    import torch
-    if workspace is None:
-        if need == 0:
-            return None, 0
-        workspace = torch.empty(need, dtype=torch.uint8, device=like.device)
-    elif not (workspace.is_cuda and workspace.device == like.device and workspace.is_contiguous()):
-        raise ValueError(f"workspace must be a contiguous tensor on {like.device}")
-    return workspace, workspace.numel() * workspace.element_size()
-
-
-def _on(t):
-    """The device of `t` made current for a call."""
-    import torch
-    return torch.cuda.device(t.device)
+def _dense_ptr(name, t, dtype, shape, device):
+    """The address of an optional contiguous tensor."""
+    if t is None:
+        return None
+    if t.dtype != dtype or t.shape != shape or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor {tuple(shape)} on {device}")
+    return t.data_ptr()
 
 
 def _steps(t):
     """Strides of all but the last dimension; 0 where there is nothing to step
     over."""
     return [s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape[:-1])]
+
+
+def _row_step(t):
+    return t.stride(-2) if t.shape[-2] > 1 else t.shape[-1]
+
+
+_CODES = {}
+
+
+def _enqueue(call, x, workspace, need, stream):
+    """call(workspace address, bytes, stream) on x's device, on `stream` or
+    the device's current one; a workspace of `need` bytes is allocated where
+    the call needs one and has none."""
+    import torch
+    dev = x.device
+    if dev.type != "cuda":
+        raise ValueError("tensors must be on a GPU")
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return _enqueue(call, x, workspace, need, stream)
+    if workspace is not None:
+        if workspace.device != dev or not workspace.is_contiguous():
+            raise ValueError(f"workspace must be a contiguous tensor on {dev}")
+        ptr, size = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    elif need > 0:
+        if stream is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        else:
+            with torch.cuda.stream(stream):  # freed for that stream's work only
+                workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        ptr, size = workspace.data_ptr(), need
+    else:
+        ptr, size = None, 0
+    raw = torch._C._cuda_getCurrentRawStream(dev.index) if stream is None else stream.cuda_stream
+    return call(ptr, size, raw)
+
+
+def _code(t):
+    """sv2_dtype of a tensor, or an error for other types."""
+    if not _CODES:
+        import torch
+        _CODES.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+    try:
+        return _CODES[t.dtype]
+    except KeyError:
+        raise ValueError(f"no kernel for {t.dtype}") from None
 
 
 def sliding_attention(q, k, v, out, *, left, right=0, sinks=0, scale=None, q_lens=None, kv_lens=None, lse=None,
@@ -1209,27 +1238,32 @@ def sliding_attention(q, k, v, out, *, left, right=0, sinks=0, scale=None, q_len
     sequence's own lengths.  `scale`: dim ** -0.5 when None.  Tensors may be
     strided views with a contiguous last dimension."""
     import torch
-    b, nq, h, d = q.shape
-    nk, g = k.shape[1], k.shape[2]
-    dev = q.device
-    for name, t, shape in (("q", q, (b, nq, h, d)), ("k", k, (b, nk, g, d)), ("v", v, (b, nk, g, d)),
-                           ("out", out, (b, nq, h, d))):
-        _need(name, t, q.dtype, shape, dev)
-    _need_dense("q_lens", q_lens, torch.int32, (b,), dev)
-    _need_dense("kv_lens", kv_lens, torch.int32, (b,), dev)
-    _need_dense("lse", lse, torch.float32, (b, h, nq), dev)
-    a = SlidingAttnArgs(b, nq, nk, h, g, d, torch_dtype_code(q), min(left, 2**31 - 1), min(right, 2**31 - 1), sinks,
+    shape = q.shape
+    b, nq, h, d = shape
+    _, nk, g, _ = k.shape
+    dtype, dev = q.dtype, q.device
+    _need("q", q, dtype, shape, dev)
+    _need("k", k, dtype, (b, nk, g, d), dev)
+    _need("v", v, dtype, (b, nk, g, d), dev)
+    _need("out", out, dtype, shape, dev)
+    most = 2**31 - 1
+    a = SlidingAttnArgs(b, nq, nk, h, g, d, _code(q), min(left, most), min(right, most), min(sinks, most),
                         d ** -0.5 if scale is None else scale,
                         q.data_ptr(), *_steps(q), k.data_ptr(), *_steps(k), v.data_ptr(), *_steps(v),
-                        out.data_ptr(), *_steps(out), None if q_lens is None else q_lens.data_ptr(),
-                        None if kv_lens is None else kv_lens.data_ptr(), None if lse is None else lse.data_ptr())
+                        out.data_ptr(), *_steps(out), _dense_ptr("q_lens", q_lens, torch.int32, (b,), dev),
+                        _dense_ptr("kv_lens", kv_lens, torch.int32, (b,), dev),
+                        _dense_ptr("lse", lse, torch.float32, (b, h, nq), dev))
     lib = load()
     ref = ctypes.byref(a)
-    need = check(lib.sv2_sliding_attention_workspace(ref), "sv2_sliding_attention_workspace")
-    with _on(q):
-        workspace, a.workspace_bytes = _bound_workspace(workspace, need, q)
-        a.workspace = None if workspace is None else workspace.data_ptr()
-        check(lib.sv2_sliding_attention(ref, _stream(stream)), "sv2_sliding_attention")
+    need = lib.sv2_sliding_attention_workspace(ref)
+    if need < 0:
+        check(need, "sv2_sliding_attention_workspace")
+
+    def call(ptr, size, raw):
+        a.workspace, a.workspace_bytes = ptr, size
+        return lib.sv2_sliding_attention(ref, raw)
+
+    check(_enqueue(call, q, workspace, need, stream), "sv2_sliding_attention")
     return out
 
 
@@ -1238,19 +1272,21 @@ def group_norm(x, y, groups, *, gamma=None, beta=None, eps=1e-5, activation=ACT_
     channels], per image and group (sv2_group_norm).  gamma, beta: fp32
     [channels] or None; y may be x."""
     import torch
-    n, rows, c = x.shape
-    _need("x", x, x.dtype, (n, rows, c), x.device)
-    _need("y", y, x.dtype, (n, rows, c), x.device)
-    _need_dense("gamma", gamma, torch.float32, (c,), x.device)
-    _need_dense("beta", beta, torch.float32, (c,), x.device)
+    shape = x.shape
+    n, rows, c = shape
+    dev = x.device
+    _need("x", x, x.dtype, shape, dev)
+    _need("y", y, x.dtype, shape, dev)
+    gp = _dense_ptr("gamma", gamma, torch.float32, (c,), dev)
+    bp = _dense_ptr("beta", beta, torch.float32, (c,), dev)
     lib = load()
-    code = torch_dtype_code(x)
-    need = check(lib.sv2_group_norm_workspace(code, n, rows, c, groups), "sv2_group_norm_workspace")
-    with _on(x):
-        workspace, size = _bound_workspace(workspace, need, x)
-        check(lib.sv2_group_norm(_ptr(x), x.stride(0), x.stride(1) if rows > 1 else c, _ptr(y), y.stride(0),
-                                 y.stride(1) if rows > 1 else c, code, n, rows, c, groups, eps, _ptr(gamma),
-                                 _ptr(beta), activation, _ptr(workspace), size, _stream(stream)), "sv2_group_norm")
+    code = _code(x)
+    need = lib.sv2_group_norm_workspace(code, n, rows, c, groups)
+    if need < 0:
+        check(need, "sv2_group_norm_workspace")
+    check(_enqueue(lambda ptr, size, raw: lib.sv2_group_norm(
+        x.data_ptr(), x.stride(0), _row_step(x), y.data_ptr(), y.stride(0), _row_step(y), code, n, rows, c, groups,
+        eps, gp, bp, activation, ptr, size, raw), x, workspace, need, stream), "sv2_group_norm")
     return y
 
 
@@ -1261,25 +1297,27 @@ def linear(x, w, y, *, bias=None, activation=ACT_NONE, residual=None, workspace=
     import torch
     rows, k = x.shape
     n = w.shape[0]
-    for name, t, shape in (("x", x, (rows, k)), ("w", w, (n, k)), ("y", y, (rows, n))):
-        _need(name, t, x.dtype, shape, x.device)
-    _need_dense("bias", bias, torch.float32, (n,), x.device)
+    dtype, dev = x.dtype, x.device
+    _need("x", x, dtype, (rows, k), dev)
+    _need("w", w, dtype, (n, k), dev)
+    _need("y", y, dtype, (rows, n), dev)
     if residual is not None:
-        _need("residual", residual, x.dtype, (rows, n), x.device)
-
-    def step(t):
-        return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-    a = LinearArgs(rows, k, n, torch_dtype_code(x), activation, x.data_ptr(), step(x), w.data_ptr(), step(w),
-                   None if bias is None else bias.data_ptr(), None if residual is None else residual.data_ptr(),
-                   0 if residual is None else step(residual), y.data_ptr(), step(y))
+        _need("residual", residual, dtype, (rows, n), dev)
+    a = LinearArgs(rows, k, n, _code(x), activation, x.data_ptr(), _row_step(x), w.data_ptr(), _row_step(w),
+                   _dense_ptr("bias", bias, torch.float32, (n,), dev),
+                   None if residual is None else residual.data_ptr(), 0 if residual is None else _row_step(residual),
+                   y.data_ptr(), _row_step(y))
     lib = load()
     ref = ctypes.byref(a)
-    need = check(lib.sv2_linear_workspace(ref), "sv2_linear_workspace")
-    with _on(x):
-        workspace, a.workspace_bytes = _bound_workspace(workspace, need, x)
-        a.workspace = None if workspace is None else workspace.data_ptr()
-        check(lib.sv2_linear(ref, _stream(stream)), "sv2_linear")
+    need = lib.sv2_linear_workspace(ref)
+    if need < 0:
+        check(need, "sv2_linear_workspace")
+
+    def call(ptr, size, raw):
+        a.workspace, a.workspace_bytes = ptr, size
+        return lib.sv2_linear(ref, raw)
+
+    check(_enqueue(call, x, workspace, need, stream), "sv2_linear")
     return y
 
 
