@@ -3,7 +3,18 @@
 //   y[m][n] = act(sum_k x[m][k] w[n][k] + bias[n]) + residual[m][n]
 //
 // fp16 or bf16 operands, fp32 sums, one rounding at the end.  Any sizes, row
-// strides and element alignment.
+// strides and element alignment.  The product is computed transposed (w as the
+// first operand of v_mfma_f32_16x16x32), so a lane holds four consecutive
+// columns of one output row.
+//
+// Two forms, by the number of rows.
+//   few   up to 64 rows: a stream of w.  A workgroup of four waves takes 16 CT
+//         columns and splits K among its waves in blocks of 64 (interleaved:
+//         together they read 512 consecutive bytes of a row).  Each wave
+//         fetches whole 128-byte lines of w and x straight into a ring of LDS
+//         slots of its own, so no barrier stands in the stream; the four
+//         partial sums meet in LDS at the end.  One launch, no workspace.
+//   any   more rows: 128 x 128 tiles through registers.
 #include "sv2_internal.h"
 #include "activation.h"
 #include "vec_io.h"
@@ -51,6 +62,7 @@ struct LinearParams
     const float* bias;
     long long ldx, ldw, ldy, ldr;
     int m, n, k;
+    int act;
     int tiles_m, tiles_n;
     int vec4; // rows of y and the residual hold whole aligned groups of 4
 };
@@ -73,8 +85,8 @@ __device__ inline u4 load8(const uint16_t* row, int k, int k_end)
 }
 
 // Four columns of one output row.
-template <typename IO, int ACT>
-__device__ inline void finish4(const LinearParams& p, int m, int n, f4 v)
+template <typename IO, typename A>
+__device__ inline void finish4(const LinearParams& p, int m, int n, f4 v, A act)
 {
     if (m >= p.m || n >= p.n)
         return;
@@ -92,7 +104,7 @@ __device__ inline void finish4(const LinearParams& p, int m, int n, f4 v)
             float t = v[e];
             if (p.bias)
                 t += p.bias[n + e];
-            t = activate<ACT, false>(t);
+            t = act(t);
             if (r)
                 t += IO::to_float(static_cast<uint16_t>(old[e >> 1] >> (16 * (e & 1))));
             o[e] = IO::from_float(t);
@@ -107,16 +119,195 @@ __device__ inline void finish4(const LinearParams& p, int m, int n, f4 v)
             float t = v[e];
             if (p.bias)
                 t += p.bias[n + e];
-            t = activate<ACT, false>(t);
+            t = act(t);
             if (r)
                 t += IO::to_float(r[e]);
             y[e] = IO::from_float(t);
         }
 }
 
+// The activation by a uniform branch, for epilogues that are a small part of
+// their kernel.
+__device__ inline float activate_by(int act, float v)
+{
+    switch (act)
+    {
+    case SV2_ACT_SILU: return activate<SV2_ACT_SILU, false>(v);
+    case SV2_ACT_GELU: return activate<SV2_ACT_GELU, false>(v);
+    case SV2_ACT_GELU_TANH: return activate<SV2_ACT_GELU_TANH, false>(v);
+    default: return v;
+    }
+}
+
+// 16 bytes per lane from global memory (uniform base + 32-bit lane offset)
+// straight into LDS at lds + 16 * lane (lds wave-uniform, in M0; one wait
+// state between the write of M0 and its use).  The compiler does not count
+// these loads; the loop waits for them itself.
+__device__ inline void dma16(const void* base, unsigned voff, unsigned lds)
+{
+    const unsigned long long b = reinterpret_cast<unsigned long long>(base);
+    const unsigned lo = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(b));
+    const unsigned hi = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(b >> 32));
+    lds = __builtin_amdgcn_readfirstlane(lds);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :
+                 : "s"(lds), "v"(voff), "s"(static_cast<unsigned long long>(hi) << 32 | lo)
+                 : "memory", "m0");
+}
+
+template <int N>
+__device__ inline void wait_vm()
+{
+    static_assert(N >= 0 && N < 64, "vmcnt holds 6 bits");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+constexpr int kFewWaves = 4;
+constexpr int kFewRows = 64;
+
+// The few form's LDS: a ring of slots of 16 CT rows of w and 16 MT rows of x,
+// 128 bytes each, per wave; 16-byte chunk c of row r sits in slot c ^ (r & 7),
+// so the 16 rows an operand read takes at one chunk fall on different banks.
+// Two workgroups a CU where three blocks ahead fit, else one.
+template <int MT, int CT>
+struct FewShape
+{
+    static constexpr int kSlot = (MT + CT) * 2048;
+    static constexpr int kPer = 2 * (MT + CT); // fetches of a block
+    static constexpr int kBudget = (80 * 1024 / (kFewWaves * kSlot) >= 4 ? 80 : 160) * 1024;
+    static constexpr int kFit = kBudget / (kFewWaves * kSlot);
+    static constexpr int kSlots = kFit > 6 ? 6 : kFit;
+    static constexpr int kLds = kFewWaves * kSlots * kSlot;
+    static_assert(kSlots >= 2 && MT * CT * 1024 <= kSlots * kSlot, "a wave's sums fit its ring");
+};
+
+// `WHOLE`: operands in 16-byte pieces (pointers 16-byte aligned, strides of w
+// and x multiples of 8); else every piece is loaded through registers.
+template <typename IO, int MT, int CT, bool WHOLE>
+__global__ __launch_bounds__(64 * kFewWaves) void linear_few_kernel(LinearParams p)
+{
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    using S = FewShape<MT, CT>;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lr = lane & 15;
+    const int lq = lane >> 4;
+    const int n0 = blockIdx.x * 16 * CT;
+    f4 acc[CT][MT];
+#pragma unroll
+    for (int c = 0; c < CT; c++)
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+            acc[c][m] = f4{0.f, 0.f, 0.f, 0.f};
+    char* ring = smem + wave * S::kSlots * S::kSlot;
+    // rows past the end repeat the last one; their sums are not stored
+    int done = 0; // k that the stream has taken
+    if constexpr (WHOLE)
+    {
+        const int blocks = p.k / 64;
+        done = blocks * 64;
+        const int mine = wave < blocks ? (blocks - 1 - wave) / kFewWaves + 1 : 0;
+        const char* wb = reinterpret_cast<const char*>(p.w + n0 * p.ldw) + 128 * wave;
+        const char* xb = reinterpret_cast<const char*>(p.x) + 128 * wave;
+        const int fr = lane >> 3;
+        const unsigned chunk = ((lane & 7) ^ fr) << 4;
+        unsigned wo[2 * CT], xo[2 * MT];
+#pragma unroll
+        for (int i = 0; i < 2 * CT; i++)
+            wo[i] = static_cast<unsigned>(min(8 * i + fr, p.n - 1 - n0) * p.ldw * 2) + chunk;
+#pragma unroll
+        for (int i = 0; i < 2 * MT; i++)
+            xo[i] = static_cast<unsigned>(min(8 * i + fr, p.m - 1) * p.ldx * 2) + chunk;
+        const unsigned lds = static_cast<unsigned>(reinterpret_cast<size_t>(ring));
+        int slot = 0;
+        auto fetch = [&]() {
+            const unsigned d = lds + slot * S::kSlot;
+#pragma unroll
+            for (int i = 0; i < 2 * CT; i++)
+                dma16(wb, wo[i], d + 1024 * i);
+#pragma unroll
+            for (int i = 0; i < 2 * MT; i++)
+                dma16(xb, xo[i], d + CT * 2048 + 1024 * i);
+            wb += 128 * kFewWaves;
+            xb += 128 * kFewWaves;
+            slot = slot + 1 == S::kSlots ? 0 : slot + 1;
+        };
+        unsigned at[2];
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+            at[s] = lr * 128 + (((4 * s + lq) ^ (lr & 7)) << 4);
+        const char* st = ring;
+        auto multiply = [&]() {
+#pragma unroll
+            for (int s = 0; s < 2; s++)
+            {
+                u4 a[CT], b[MT];
+#pragma unroll
+                for (int c = 0; c < CT; c++)
+                    a[c] = *reinterpret_cast<const u4*>(st + at[s] + 2048 * c);
+#pragma unroll
+                for (int m = 0; m < MT; m++)
+                    b[m] = *reinterpret_cast<const u4*>(st + at[s] + 2048 * (CT + m));
+#pragma unroll
+                for (int c = 0; c < CT; c++)
+#pragma unroll
+                    for (int m = 0; m < MT; m++)
+                        acc[c][m] = IO::mfma(a[c], b[m], acc[c][m]);
+            }
+            st = st + S::kSlot == ring + S::kSlots * S::kSlot ? ring : st + S::kSlot;
+        };
+        for (int i = 0; i < min(mine, S::kSlots - 1); i++)
+            fetch();
+        int i = 0;
+        for (; i + S::kSlots - 1 < mine; i++)
+        {
+            // the slot multiplied before is free once its reads are done
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            fetch();
+            wait_vm<(S::kSlots - 1) * S::kPer>();
+            multiply();
+        }
+        wait_vm<0>();
+        for (; i < mine; i++)
+            multiply();
+    }
+    // what the stream left: the last k of all (WHOLE), or everything
+    for (int k0 = done + 32 * wave; k0 < p.k; k0 += 32 * kFewWaves)
+    {
+        u4 a[CT], b[MT];
+#pragma unroll
+        for (int c = 0; c < CT; c++)
+            a[c] = load8(p.w + min(n0 + 16 * c + lr, p.n - 1) * p.ldw, k0 + 8 * lq, p.k);
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+            b[m] = load8(p.x + min(16 * m + lr, p.m - 1) * p.ldx, k0 + 8 * lq, p.k);
+#pragma unroll
+        for (int c = 0; c < CT; c++)
+#pragma unroll
+            for (int m = 0; m < MT; m++)
+                acc[c][m] = IO::mfma(a[c], b[m], acc[c][m]);
+    }
+    // the waves' sums, added in wave order
+    f4* sums = reinterpret_cast<f4*>(ring);
+#pragma unroll
+    for (int c = 0; c < CT; c++)
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+            sums[(c * MT + m) * 64 + lane] = acc[c][m];
+    __syncthreads();
+    for (int t = wave; t < CT * MT; t += kFewWaves)
+    {
+        f4 v = reinterpret_cast<const f4*>(smem)[t * 64 + lane];
+#pragma unroll
+        for (int w = 1; w < kFewWaves; w++)
+            v += reinterpret_cast<const f4*>(smem + w * S::kSlots * S::kSlot)[t * 64 + lane];
+        const int c = t / MT;
+        finish4<IO>(p, 16 * (t - c * MT) + lr, n0 + 16 * c + 4 * lq, v, [&](float x) { return activate_by(p.act, x); });
+    }
+}
+
 // 128 x 128 outputs by 4 waves of 64 x 64, K in steps of 32 through registers
-// into two LDS buffers; the product is computed transposed (w as the first
-// operand), so a lane holds four columns of one output row.
+// into two LDS buffers.
 template <typename IO, int ACT>
 __global__ __launch_bounds__(256, 2) void linear_any_kernel(LinearParams p)
 {
@@ -196,7 +387,8 @@ __global__ __launch_bounds__(256, 2) void linear_any_kernel(LinearParams p)
     for (int t = 0; t < 4; t++)
 #pragma unroll
         for (int u = 0; u < 4; u++)
-            finish4<IO, ACT>(p, m0 + wm + 16 * u + lr, n0 + wn + 16 * t + 4 * lq, acc[t][u]);
+            finish4<IO>(p, m0 + wm + 16 * u + lr, n0 + wn + 16 * t + 4 * lq, acc[t][u],
+                        [](float v) { return activate<ACT, false>(v); });
 }
 
 template <typename IO, int ACT>
@@ -210,6 +402,33 @@ int run_linear(LinearParams p, hipStream_t stream)
     hipLaunchKernelGGL((linear_any_kernel<IO, ACT>), dim3(static_cast<unsigned>(total)), dim3(256), 0, stream, p);
     const hipError_t err = hipGetLastError();
     return err == hipSuccess ? SV2_OK : hip_error(err, "sv2_linear launch");
+}
+
+template <typename IO, int MT, int CT, bool WHOLE>
+int run_few(const LinearParams& p, hipStream_t stream)
+{
+    constexpr int kLds = FewShape<MT, CT>::kLds;
+    const int rc = set_dynamic_lds(reinterpret_cast<const void*>(&linear_few_kernel<IO, MT, CT, WHOLE>), kLds,
+                                   "linear_few: dynamic LDS attribute");
+    if (rc != SV2_OK)
+        return rc;
+    const unsigned grid = static_cast<unsigned>((p.n + 16LL * CT - 1) / (16 * CT));
+    hipLaunchKernelGGL((linear_few_kernel<IO, MT, CT, WHOLE>), dim3(grid), dim3(64 * kFewWaves), kLds, stream, p);
+    const hipError_t err = hipGetLastError();
+    return err == hipSuccess ? SV2_OK : hip_error(err, "sv2_linear launch");
+}
+
+template <typename IO, bool WHOLE>
+int run_few_rows(const LinearParams& p, hipStream_t stream)
+{
+    if (p.m <= 16)
+        return run_few<IO, 1, 1, WHOLE>(p, stream);
+    if (p.m <= 32)
+        return run_few<IO, 2, 1, WHOLE>(p, stream);
+    // x is read once for every 16 CT columns
+    if (p.n >= 64 * 160)
+        return run_few<IO, 4, 4, WHOLE>(p, stream);
+    return run_few<IO, 4, 1, WHOLE>(p, stream);
 }
 
 template <typename IO>
@@ -283,6 +502,16 @@ try
     p.k = a.in;
     p.vec4 = p.n % 4 == 0 && p.ldy % 4 == 0 && p.ldr % 4 == 0 && !misaligned(p.y, 8) && !misaligned(p.r, 8);
     const hipStream_t st = static_cast<hipStream_t>(stream);
+    p.act = a.activation;
+    // pieces of 16 bytes: the rows a workgroup fetches lie within 32-bit offsets
+    const bool whole = p.ldx % 8 == 0 && p.ldw % 8 == 0 && !misaligned(p.x, 16) && !misaligned(p.w, 16) &&
+                       std::max(p.ldx, p.ldw) < (1LL << 31) / (2 * kFewRows);
+    if (p.m <= kFewRows)
+    {
+        if (a.dtype == SV2_F16)
+            return whole ? run_few_rows<HalfIO, true>(p, st) : run_few_rows<HalfIO, false>(p, st);
+        return whole ? run_few_rows<BfloatIO, true>(p, st) : run_few_rows<BfloatIO, false>(p, st);
+    }
     return a.dtype == SV2_F16 ? run_act<HalfIO>(p, a.activation, st) : run_act<BfloatIO>(p, a.activation, st);
 }
 catch (...)
