@@ -43,6 +43,7 @@ struct NormArgs
     const float* gamma;
     const float* beta;
     int rows, channels, groups, width;
+    int unit;                 // channels of a thread's V that surely share a group: gcd(width, V)
     float eps;
     int slab_groups, slabs;   // slab form
     int chunk_rows, chunks;   // rows form
@@ -117,32 +118,66 @@ constexpr int wide()
     return 16 / elem_bytes<T>();
 }
 
-__device__ inline float wave_sum(float v)
+// Over the `team` lanes (a power of two) that share lane / team.
+__device__ inline float team_sum(float v, int team)
 {
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1)
+    for (int d = team >> 1; d > 0; d >>= 1)
         v += __shfl_xor(v, d, 64);
     return v;
 }
 
-// Joins `entries` pieces (count n(e), mean, M2) whose counts add up to `total`,
-// one wave; every lane receives the result.
-template <typename N, typename M, typename S>
-__device__ inline void join(int entries, float total, int lane, N n, M mean, S m2, float* out_mean, float* out_m2)
+// Joins `entries` pieces (count n(e), mean, M2) whose counts add up to `total`
+// by a team of lanes, `lane` being the caller's place in it; every lane
+// receives the result.
+template <typename N, typename E>
+__device__ inline void join(int entries, float total, int team, int lane, N n, E entry, float* out_mean, float* out_m2)
 {
-    const float ref = mean(0);
+    const float ref = entry(0).x;
     float d = 0.f;
-    for (int e = lane; e < entries; e += 64)
-        d += n(e) * (mean(e) - ref);
-    const float mu = ref + wave_sum(d) / total;
+    for (int e = lane; e < entries; e += team)
+        d += n(e) * (entry(e).x - ref);
+    const float mu = ref + team_sum(d, team) / total;
     float s = 0.f;
-    for (int e = lane; e < entries; e += 64)
+    for (int e = lane; e < entries; e += team)
     {
-        const float off = mean(e) - mu;
-        s += m2(e) + n(e) * off * off;
+        const float2 p = entry(e);
+        const float off = p.x - mu;
+        s += p.y + n(e) * off * off;
     }
     *out_mean = mu;
-    *out_m2 = wave_sum(s);
+    *out_m2 = team_sum(s, team);
+}
+
+// Lanes per group, so that a workgroup's threads take its groups at once
+// where they can.
+__device__ inline int team_of(int threads, int groups)
+{
+    int team = 64;
+    while (team > 1 && threads / team < groups)
+        team >>= 1;
+    return team;
+}
+
+// Joins the V channels' pieces (each over n rows) by spans of `unit` channels,
+// which lie in one group, and writes one piece a span.
+template <int V>
+__device__ inline void put_pieces(float2* to, float mean[V], float m2[V], float n, int unit)
+{
+#pragma unroll
+    for (int span = 1; span < V; span *= 2)
+        if (span < unit)
+#pragma unroll
+            for (int e = 0; e < V; e += 2 * span)
+            {
+                const float d = mean[e + span] - mean[e];
+                mean[e] += 0.5f * d;
+                m2[e] += m2[e + span] + d * d * (0.5f * n * static_cast<float>(span));
+            }
+    int k = 0;
+#pragma unroll
+    for (int e = 0; e < V; e++)
+        if ((e & (unit - 1)) == 0)
+            to[k++] = make_float2(mean[e], m2[e]);
 }
 
 // Rows of 0 .. rows - 1 that row lane r of `lanes` takes.
@@ -230,28 +265,25 @@ __global__ __launch_bounds__(kSlabThreads) void norm_slab_kernel(NormArgs p)
             for (int e = 0; e < V; e++)
                 m2[e] += (x[e] - mean[e]) * (x[e] - mean[e]);
         }
-    float* s_mean = smem;
-    float* s_m2 = smem + lanes * sc;
-    float2* s_stat = reinterpret_cast<float2*>(smem + 2 * lanes * sc);
+    // pieces [row lane][span of unit channels], then (mean, rstd) per group
+    const int unit = p.unit;
+    const int spans = sc / unit;
+    float2* s_piece = reinterpret_cast<float2*>(smem);
+    float2* s_stat = s_piece + lanes * spans;
     if (active)
-#pragma unroll
-        for (int e = 0; e < V; e++)
-        {
-            s_mean[r0 * sc + c + e] = mean[e];
-            s_m2[r0 * sc + c + e] = m2[e];
-        }
+        put_pieces<V>(s_piece + r0 * spans + c / unit, mean, m2, static_cast<float>(mine), unit);
     __syncthreads();
-    const int wave = threadIdx.x >> 6;
     const int used = min(lanes, p.rows); // row lanes that hold a row
     const float total = static_cast<float>(p.rows) * static_cast<float>(p.width);
-    for (int g = wave; g < ng; g += blockDim.x >> 6)
+    const int team = team_of(blockDim.x, ng);
+    const int per = p.width / unit;
+    for (int g = threadIdx.x / team; g < ng; g += blockDim.x / team)
     {
-        auto at = [&](int e) { const int r = e / p.width; return r * sc + g * p.width + (e - r * p.width); };
         float mu, s;
-        join(used * p.width, total, threadIdx.x & 63,
-             [&](int e) { return static_cast<float>(lane_rows(p.rows, lanes, e / p.width)); },
-             [&](int e) { return s_mean[at(e)]; }, [&](int e) { return s_m2[at(e)]; }, &mu, &s);
-        if ((threadIdx.x & 63) == 0)
+        join(used * per, total, team, threadIdx.x & (team - 1),
+             [&](int e) { return static_cast<float>(lane_rows(p.rows, lanes, e / per) * unit); },
+             [&](int e) { const int r = e / per; return s_piece[r * spans + g * per + (e - r * per)]; }, &mu, &s);
+        if ((threadIdx.x & (team - 1)) == 0)
             s_stat[g] = make_float2(mu, 1.f / sqrtf(s / total + p.eps));
     }
     __syncthreads();
@@ -303,8 +335,8 @@ __global__ __launch_bounds__(kRowThreads) void norm_stats_kernel(NormArgs p)
     const int first = chunk * p.chunk_rows;
     const int rows = min(p.chunk_rows, p.rows - first);
     const Columns k = columns<V>(p.channels);
-    float* s_mean = smem;
-    float* s_m2 = smem + k.lanes * p.channels;
+    const int spans = p.channels / p.unit;
+    float2* s_piece = reinterpret_cast<float2*>(smem); // [row lane][span of unit channels]
     for (int round = 0; round < k.rounds; round++)
     {
         const int r0 = k.rounds > 1 ? 0 : threadIdx.x / k.nc;
@@ -377,25 +409,20 @@ __global__ __launch_bounds__(kRowThreads) void norm_stats_kernel(NormArgs p)
                 m2[e] += d * (x[e] - mean[e]);
             }
         }
-#pragma unroll
-        for (int e = 0; e < V; e++)
-        {
-            s_mean[r0 * p.channels + col * V + e] = mean[e];
-            s_m2[r0 * p.channels + col * V + e] = m2[e];
-        }
+        put_pieces<V>(s_piece + r0 * spans + col * V / p.unit, mean, m2, static_cast<float>(mine), p.unit);
     }
     __syncthreads();
     const int used = min(k.lanes, rows);
     const float total = static_cast<float>(rows) * static_cast<float>(p.width);
-    const int lane = threadIdx.x & 63;
-    for (int g = threadIdx.x >> 6; g < p.groups; g += kRowThreads >> 6)
+    const int team = team_of(kRowThreads, p.groups);
+    const int per = p.width / p.unit;
+    for (int g = threadIdx.x / team; g < p.groups; g += kRowThreads / team)
     {
-        auto at = [&](int e) { const int r = e / p.width; return r * p.channels + g * p.width + (e - r * p.width); };
         float mu, s;
-        join(used * p.width, total, lane,
-             [&](int e) { return static_cast<float>(lane_rows(rows, k.lanes, e / p.width)); },
-             [&](int e) { return s_mean[at(e)]; }, [&](int e) { return s_m2[at(e)]; }, &mu, &s);
-        if (lane == 0)
+        join(used * per, total, team, threadIdx.x & (team - 1),
+             [&](int e) { return static_cast<float>(lane_rows(rows, k.lanes, e / per) * p.unit); },
+             [&](int e) { const int r = e / per; return s_piece[r * spans + g * per + (e - r * per)]; }, &mu, &s);
+        if ((threadIdx.x & (team - 1)) == 0)
             p.part[(static_cast<long long>(image) * p.groups + g) * p.chunks + chunk] = make_float2(mu, s);
     }
 }
@@ -407,9 +434,9 @@ __global__ __launch_bounds__(64) void norm_join_kernel(NormArgs p)
     const float w = static_cast<float>(p.width);
     const float total = static_cast<float>(p.rows) * w;
     float mu, s;
-    join(p.chunks, total, threadIdx.x,
+    join(p.chunks, total, 64, threadIdx.x,
          [&](int e) { return w * static_cast<float>(min(p.chunk_rows, p.rows - e * p.chunk_rows)); },
-         [&](int e) { return part[e].x; }, [&](int e) { return part[e].y; }, &mu, &s);
+         [&](int e) { return part[e]; }, &mu, &s);
     if (threadIdx.x == 0)
         p.stat[blockIdx.x] = make_float2(mu, 1.f / sqrtf(s / total + p.eps));
 }
@@ -635,6 +662,9 @@ try
     const bool one_image = images == 1; // its image strides are not read
     const bool wide = channels % v == 0 && x_row_stride % v == 0 && y_row_stride % v == 0 && !misaligned(x, 16) &&
                       !misaligned(y, 16) && (one_image || (x_image_stride % v == 0 && y_image_stride % v == 0));
+    p.unit = 1;
+    while (wide && p.unit < v && p.width % (2 * p.unit) == 0)
+        p.unit *= 2;
     const Slab s = plan_slab(p, wide ? v : 1, wide ? kKeepWide : kKeepOne, bytes);
     const bool slab = s.threads > 0;
     if (!slab)
