@@ -45,7 +45,7 @@ struct NormArgs
     int rows, channels, groups, width;
     int unit;                 // channels of a thread's V that surely share a group: gcd(width, V)
     float eps;
-    int slab_groups, slabs;   // slab form
+    int slab_groups, slabs, blocks; // slab form
     int chunk_rows, chunks;   // rows form
     float2* part;             // rows form: (mean, M2) [image][group][chunk], then (mean, rstd) [image][group]
     float2* stat;
@@ -59,6 +59,17 @@ template <typename T>
 constexpr int elem_bytes()
 {
     return std::is_same_v<T, F32> ? 4 : 2;
+}
+
+typedef __attribute__((ext_vector_type(4))) unsigned u4;
+
+// Outputs go past the caches: written through the last-level cache they leave
+// dirty lines there, whose eviction costs the statistics of the next call half
+// of their rate (3 x 230400 x 256 bf16: statistics 85 against 58 us, the whole
+// 213 against 193).
+__device__ inline void put16(void* to, u4 v)
+{
+    __builtin_nontemporal_store(v, static_cast<u4*>(to));
 }
 
 // V elements of one row piece, as loaded.
@@ -94,7 +105,27 @@ struct Piece<T, 8>
     Raw8<T> r;
     __device__ void load(const void* base, long long i) { ld_raw8<T>(base, i, r); }
     __device__ void get(float x[8]) const { raw8_float(r, x); }
-    __device__ static void store(void* base, long long i, const float x[8]) { st8<T>(base, i, x); }
+    __device__ static void store(void* base, long long i, const float x[8])
+    {
+        if constexpr (std::is_same_v<T, BF16>)
+        {
+            // v_cvt_pk_bf16_f32 (nearest even)
+            typedef __attribute__((ext_vector_type(8))) __bf16 b8;
+            b8 v;
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                v[e] = static_cast<__bf16>(x[e]);
+            put16(static_cast<uint16_t*>(base) + i, __builtin_bit_cast(u4, v));
+        }
+        else
+        {
+            f16x8 v;
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                v[e] = static_cast<_Float16>(x[e]);
+            put16(static_cast<uint16_t*>(base) + i, __builtin_bit_cast(u4, v));
+        }
+    }
 };
 template <>
 struct Piece<F32, 4>
@@ -107,7 +138,8 @@ struct Piece<F32, 4>
     }
     __device__ static void store(void* base, long long i, const float x[4])
     {
-        *reinterpret_cast<float4*>(static_cast<float*>(base) + i) = make_float4(x[0], x[1], x[2], x[3]);
+        typedef __attribute__((ext_vector_type(4))) float f4;
+        put16(static_cast<float*>(base) + i, __builtin_bit_cast(u4, f4{x[0], x[1], x[2], x[3]}));
     }
 };
 
@@ -180,28 +212,45 @@ __device__ inline void put_pieces(float2* to, float mean[V], float m2[V], float 
             to[k++] = make_float2(mean[e], m2[e]);
 }
 
-// Rows of 0 .. rows - 1 that row lane r of `lanes` takes.
-__device__ inline int lane_rows(int rows, int lanes, int r)
+// How `rows` rows fall to row lanes: lane r takes rows r, r + lanes, ...
+struct Share
 {
-    return r < rows ? (rows - 1 - r) / lanes + 1 : 0;
+    int each, more; // lanes 0 .. more - 1 take one row more
+    __device__ Share(int rows, int lanes) : each(rows / lanes), more(rows - each * lanes) {}
+    __device__ int of(int r) const { return each + (r < more ? 1 : 0); }
+};
+
+// e / d for 0 <= e < 2^21 (pieces in LDS) and inv = 1 / d: the half keeps the
+// quotient's rounding errors, 2^-22 of it, from reaching a whole number.
+__device__ inline int quick_div(int e, float inv)
+{
+    return static_cast<int>((static_cast<float>(e) + 0.5f) * inv);
 }
 
-// gamma and beta of V channels, with the group's mean and 1 / sqrt(var + eps)
-// folded into the scale.
+// gamma and beta of V channels, then with the group's mean and
+// 1 / sqrt(var + eps) folded into the scale.
 template <int V>
 struct Affine
 {
     float mean[V], a[V], b[V];
-    template <typename G>
-    __device__ void load(const NormArgs& p, int c0, G stat)
+    __device__ void load(const float* gamma, const float* beta, int c0)
     {
 #pragma unroll
         for (int e = 0; e < V; e++)
         {
-            const float2 s = stat(c0 + e);
+            a[e] = gamma ? gamma[c0 + e] : 1.f;
+            b[e] = beta ? beta[c0 + e] : 0.f;
+        }
+    }
+    template <typename G>
+    __device__ void scale(G stat)
+    {
+#pragma unroll
+        for (int e = 0; e < V; e++)
+        {
+            const float2 s = stat(e);
             mean[e] = s.x;
-            a[e] = s.y * (p.gamma ? p.gamma[c0 + e] : 1.f);
-            b[e] = p.beta ? p.beta[c0 + e] : 0.f;
+            a[e] *= s.y;
         }
     }
     template <int ACT, bool EXACT>
@@ -219,8 +268,13 @@ template <typename T, int V, int KEEP, int ACT>
 __global__ __launch_bounds__(kSlabThreads) void norm_slab_kernel(NormArgs p)
 {
     extern __shared__ __attribute__((aligned(16))) float smem[];
-    const int image = blockIdx.x / p.slabs;
-    const int g0 = (blockIdx.x - image * p.slabs) * p.slab_groups;
+    // XCD x (workgroup id mod 8) takes a contiguous run: slabs that share a
+    // 128-byte line share an L2
+    const int id = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+    if (id >= p.blocks)
+        return;
+    const int image = id / p.slabs;
+    const int g0 = (id - image * p.slabs) * p.slab_groups;
     const int ng = min(p.slab_groups, p.groups - g0);
     const int c_base = g0 * p.width;
     const int sc = ng * p.width;     // channels of this slab, a multiple of V
@@ -229,7 +283,8 @@ __global__ __launch_bounds__(kSlabThreads) void norm_slab_kernel(NormArgs p)
     const int r0 = threadIdx.x / nc;
     const int c = (threadIdx.x - r0 * nc) * V;
     const bool active = r0 < lanes;
-    const int mine = active ? lane_rows(p.rows, lanes, r0) : 0;
+    const Share share(p.rows, lanes);
+    const int mine = active ? share.of(r0) : 0;
     const long long xi = image * p.x_image + c_base + c;
 
     Piece<T, V> keep[KEEP];
@@ -237,6 +292,9 @@ __global__ __launch_bounds__(kSlabThreads) void norm_slab_kernel(NormArgs p)
     for (int k = 0; k < KEEP; k++)
         if (k < mine)
             keep[k].load(p.x, xi + static_cast<long long>(r0 + k * lanes) * p.x_row);
+    Affine<V> f;
+    if (active)
+        f.load(p.gamma, p.beta, c_base + c);
     float mean[V], m2[V];
 #pragma unroll
     for (int e = 0; e < V; e++)
@@ -277,25 +335,20 @@ __global__ __launch_bounds__(kSlabThreads) void norm_slab_kernel(NormArgs p)
     const float total = static_cast<float>(p.rows) * static_cast<float>(p.width);
     const int team = team_of(blockDim.x, ng);
     const int per = p.width / unit;
+    const float inv_per = 1.f / static_cast<float>(per);
     for (int g = threadIdx.x / team; g < ng; g += blockDim.x / team)
     {
         float mu, s;
         join(used * per, total, team, threadIdx.x & (team - 1),
-             [&](int e) { return static_cast<float>(lane_rows(p.rows, lanes, e / per) * unit); },
-             [&](int e) { const int r = e / per; return s_piece[r * spans + g * per + (e - r * per)]; }, &mu, &s);
+             [&](int e) { return static_cast<float>(share.of(quick_div(e, inv_per)) * unit); },
+             [&](int e) { const int r = quick_div(e, inv_per); return s_piece[r * (spans - per) + g * per + e]; }, &mu, &s);
         if ((threadIdx.x & (team - 1)) == 0)
             s_stat[g] = make_float2(mu, 1.f / sqrtf(s / total + p.eps));
     }
     __syncthreads();
     if (!active)
         return;
-    Affine<V> f;
-    {
-        NormArgs q = p;
-        q.gamma = p.gamma ? p.gamma + c_base : nullptr;
-        q.beta = p.beta ? p.beta + c_base : nullptr;
-        f.load(q, c, [&](int ch) { return s_stat[ch / p.width]; });
-    }
+    f.scale([&](int e) { return s_stat[(c + e) / p.width]; });
     const long long yi = image * p.y_image + c_base + c;
 #pragma unroll
     for (int k = 0; k < KEEP; k++)
@@ -326,7 +379,7 @@ __host__ __device__ inline Columns columns(int channels)
 
 // Rows form, first launch: workgroup (image, run of chunk_rows rows).
 template <typename T, int V>
-__global__ __launch_bounds__(kRowThreads) void norm_stats_kernel(NormArgs p)
+__global__ __launch_bounds__(kRowThreads, 4) void norm_stats_kernel(NormArgs p)
 {
     extern __shared__ __attribute__((aligned(16))) float smem[];
     constexpr int kHeld = V == 1 ? 16 : 8; // rows in registers at a time
@@ -335,6 +388,7 @@ __global__ __launch_bounds__(kRowThreads) void norm_stats_kernel(NormArgs p)
     const int first = chunk * p.chunk_rows;
     const int rows = min(p.chunk_rows, p.rows - first);
     const Columns k = columns<V>(p.channels);
+    const Share share(rows, k.lanes);
     const int spans = p.channels / p.unit;
     float2* s_piece = reinterpret_cast<float2*>(smem); // [row lane][span of unit channels]
     for (int round = 0; round < k.rounds; round++)
@@ -343,25 +397,43 @@ __global__ __launch_bounds__(kRowThreads) void norm_stats_kernel(NormArgs p)
         const int col = k.rounds > 1 ? round * kRowThreads + threadIdx.x : threadIdx.x - r0 * k.nc;
         if (r0 >= k.lanes || col >= k.nc)
             continue;
-        const int mine = lane_rows(rows, k.lanes, r0);
+        const int mine = share.of(r0);
         long long at = image * p.x_image + static_cast<long long>(first + r0) * p.x_row + col * V;
         const long long step = k.lanes * p.x_row;
         float mean[V], m2[V];
 #pragma unroll
         for (int e = 0; e < V; e++)
             mean[e] = m2[e] = 0.f;
+        // the next rows are on their way while these are summed
+        Piece<T, V> ahead[kHeld];
+        if (kHeld <= mine)
+#pragma unroll
+            for (int i = 0; i < kHeld; i++)
+                ahead[i].load(p.x, at + i * step);
         int done = 0;
         for (; done + kHeld <= mine; done += kHeld)
         {
             Piece<T, V> h[kHeld];
 #pragma unroll
             for (int i = 0; i < kHeld; i++)
-                h[i].load(p.x, at + i * step);
+                h[i] = ahead[i];
             at += kHeld * step;
-            float bm[V], bs[V];
+            if (done + 2 * kHeld <= mine)
+#pragma unroll
+                for (int i = 0; i < kHeld; i++)
+                    ahead[i].load(p.x, at + i * step);
+            // sums of differences from the mean so far (the first row at the
+            // start): the subtraction below takes at most 7/8 of s2 away, the
+            // reference being one of the values or the mean of as many
+            float ref[V], s1[V], s2[V];
+            if (done == 0)
+                h[0].get(mean);
 #pragma unroll
             for (int e = 0; e < V; e++)
-                bm[e] = bs[e] = 0.f;
+            {
+                ref[e] = mean[e];
+                s1[e] = s2[e] = 0.f;
+            }
 #pragma unroll
             for (int i = 0; i < kHeld; i++)
             {
@@ -369,28 +441,19 @@ __global__ __launch_bounds__(kRowThreads) void norm_stats_kernel(NormArgs p)
                 h[i].get(x);
 #pragma unroll
                 for (int e = 0; e < V; e++)
-                    bm[e] += x[e];
+                {
+                    const float d = x[e] - ref[e];
+                    s1[e] += d;
+                    s2[e] = __builtin_fmaf(d, d, s2[e]);
+                }
             }
-#pragma unroll
-            for (int e = 0; e < V; e++)
-                bm[e] *= 1.f / kHeld;
-#pragma unroll
-            for (int i = 0; i < kHeld; i++)
-            {
-                float x[V];
-                h[i].get(x);
-#pragma unroll
-                for (int e = 0; e < V; e++)
-                    bs[e] += (x[e] - bm[e]) * (x[e] - bm[e]);
-            }
-            const float share = static_cast<float>(kHeld) / static_cast<float>(done + kHeld);
-            const float both = share * static_cast<float>(done);
+            const float inv = 1.f / static_cast<float>(done + kHeld);
 #pragma unroll
             for (int e = 0; e < V; e++)
             {
-                const float d = bm[e] - mean[e];
-                mean[e] += d * share;
-                m2[e] += bs[e] + d * d * both;
+                const float d = s1[e] * inv;
+                mean[e] += d;
+                m2[e] += __builtin_fmaf(-d, s1[e], s2[e]);
             }
         }
         for (; done < mine; done++)
@@ -416,27 +479,70 @@ __global__ __launch_bounds__(kRowThreads) void norm_stats_kernel(NormArgs p)
     const float total = static_cast<float>(rows) * static_cast<float>(p.width);
     const int team = team_of(kRowThreads, p.groups);
     const int per = p.width / p.unit;
+    const float inv_per = 1.f / static_cast<float>(per);
     for (int g = threadIdx.x / team; g < p.groups; g += kRowThreads / team)
     {
         float mu, s;
         join(used * per, total, team, threadIdx.x & (team - 1),
-             [&](int e) { return static_cast<float>(lane_rows(rows, k.lanes, e / per) * p.unit); },
-             [&](int e) { const int r = e / per; return s_piece[r * spans + g * per + (e - r * per)]; }, &mu, &s);
+             [&](int e) { return static_cast<float>(share.of(quick_div(e, inv_per)) * p.unit); },
+             [&](int e) { const int r = quick_div(e, inv_per); return s_piece[r * (spans - per) + g * per + e]; }, &mu, &s);
         if ((threadIdx.x & (team - 1)) == 0)
             p.part[(static_cast<long long>(image) * p.groups + g) * p.chunks + chunk] = make_float2(mu, s);
     }
 }
 
-// Rows form, second launch: one wave per (image, group).
-__global__ __launch_bounds__(64) void norm_join_kernel(NormArgs p)
+// Rows form, second launch: a workgroup per (image, group), the pieces in
+// registers.
+constexpr int kJoinThreads = 256;
+constexpr int kJoinHeld = 8;
+constexpr int kMaxChunks = kJoinThreads * kJoinHeld;
+
+__device__ inline float block_sum(float v, float* scratch)
 {
+    v = team_sum(v, 64);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0)
+        scratch[threadIdx.x >> 6] = v;
+    __syncthreads();
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < kJoinThreads / 64; w++)
+        s += scratch[w];
+    return s;
+}
+
+__global__ __launch_bounds__(kJoinThreads) void norm_join_kernel(NormArgs p)
+{
+    __shared__ float scratch[kJoinThreads / 64];
     const float2* part = p.part + static_cast<long long>(blockIdx.x) * p.chunks;
     const float w = static_cast<float>(p.width);
     const float total = static_cast<float>(p.rows) * w;
-    float mu, s;
-    join(p.chunks, total, 64, threadIdx.x,
-         [&](int e) { return w * static_cast<float>(min(p.chunk_rows, p.rows - e * p.chunk_rows)); },
-         [&](int e) { return part[e]; }, &mu, &s);
+    const float ref = part[0].x;
+    float2 v[kJoinHeld];
+    float d = 0.f;
+#pragma unroll
+    for (int i = 0; i < kJoinHeld; i++)
+    {
+        const int e = threadIdx.x + kJoinThreads * i;
+        v[i] = e < p.chunks ? part[e] : make_float2(ref, 0.f);
+    }
+#pragma unroll
+    for (int i = 0; i < kJoinHeld; i++)
+    {
+        const int e = threadIdx.x + kJoinThreads * i;
+        d += w * static_cast<float>(min(p.chunk_rows, p.rows - min(e, p.chunks - 1) * p.chunk_rows)) * (v[i].x - ref);
+    }
+    const float mu = ref + block_sum(d, scratch) / total;
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < kJoinHeld; i++)
+    {
+        const int e = threadIdx.x + kJoinThreads * i;
+        const float off = v[i].x - mu;
+        if (e < p.chunks)
+            s += v[i].y + w * static_cast<float>(min(p.chunk_rows, p.rows - e * p.chunk_rows)) * off * off;
+    }
+    s = block_sum(s, scratch);
     if (threadIdx.x == 0)
         p.stat[blockIdx.x] = make_float2(mu, 1.f / sqrtf(s / total + p.eps));
 }
@@ -446,8 +552,11 @@ template <typename T, int V, int ACT>
 __global__ __launch_bounds__(kRowThreads) void norm_apply_kernel(NormArgs p)
 {
     constexpr int kHeld = V == 1 ? 16 : 8;
-    const int image = blockIdx.x / p.chunks;
-    const int first = (blockIdx.x - image * p.chunks) * p.chunk_rows;
+    // backwards: what the statistics read last may still be in the last-level
+    // cache
+    const int block = gridDim.x - 1 - blockIdx.x;
+    const int image = block / p.chunks;
+    const int first = (block - image * p.chunks) * p.chunk_rows;
     const int rows = min(p.chunk_rows, p.rows - first);
     const Columns k = columns<V>(p.channels);
     const float2* stat = p.stat + static_cast<long long>(image) * p.groups;
@@ -458,8 +567,9 @@ __global__ __launch_bounds__(kRowThreads) void norm_apply_kernel(NormArgs p)
         if (r0 >= k.lanes || col >= k.nc)
             continue;
         Affine<V> f;
-        f.load(p, col * V, [&](int ch) { return stat[ch / p.width]; });
-        const int mine = lane_rows(rows, k.lanes, r0);
+        f.load(p.gamma, p.beta, col * V);
+        f.scale([&](int e) { return stat[(col * V + e) / p.width]; });
+        const int mine = Share(rows, k.lanes).of(r0);
         long long xi = image * p.x_image + static_cast<long long>(first + r0) * p.x_row + col * V;
         long long yi = image * p.y_image + static_cast<long long>(first + r0) * p.y_row + col * V;
         const long long xs = k.lanes * p.x_row;
@@ -486,12 +596,12 @@ __global__ __launch_bounds__(kRowThreads) void norm_apply_kernel(NormArgs p)
     }
 }
 
-// The rows form's runs: enough workgroups for 256 CUs, at least 64 KB each.
+// The rows form's runs: enough workgroups for 256 CUs, at least 16 KB each.
 void plan_rows(NormArgs* p, int images, int bytes)
 {
     const long long row_bytes = static_cast<long long>(p->channels) * bytes;
-    const long long want = (static_cast<long long>(images) * p->rows + 1023) / 1024;
-    const long long least = std::max(1LL, 65536 / row_bytes);
+    const long long want = (static_cast<long long>(images) * p->rows + 2047) / 2048;
+    const long long least = std::max(1LL, 16384 / row_bytes);
     p->chunk_rows = static_cast<int>(std::min<long long>(p->rows, std::max(want, least)));
     p->chunks = (p->rows + p->chunk_rows - 1) / p->chunk_rows;
 }
@@ -502,6 +612,15 @@ long long rows_workspace(const NormArgs& p, int images)
     return static_cast<long long>(images) * p.groups * (p.chunks + 1) * static_cast<long long>(sizeof(float2));
 }
 
+// Pieces a thread of the slab form holds: 128 KB a workgroup.  Past that the
+// rows form is the faster one, though it reads twice: one image of 32 groups of
+// 16 in fp16 takes 10.0 / 14.4 / 20.3 us at 960 / 1920 / 3600 rows (61 / 123 /
+// 230 KB a workgroup) against 15.7 / 15.8 / 16.0.
+constexpr int keep_of(int v)
+{
+    return v == 1 ? 32 : 8;
+}
+
 // The slab form's shape for pieces of V elements, or threads = 0 where an
 // image does not fit: whole groups whose channels are a multiple of V, 64
 // bytes of a row at least (a quarter of the groups otherwise share a line).
@@ -509,8 +628,9 @@ struct Slab
 {
     int groups, threads, lds;
 };
-Slab plan_slab(const NormArgs& p, int v, int keep, int bytes)
+Slab plan_slab(const NormArgs& p, int v, int bytes)
 {
+    const int keep = keep_of(v);
     int g = 1;
     while (g < p.groups && (g * p.width % v != 0 || g * p.width * bytes < 64))
         g++;
@@ -530,26 +650,24 @@ Slab plan_slab(const NormArgs& p, int v, int keep, int bytes)
     return Slab{0, 0, 0};
 }
 
-constexpr int kKeepWide = 8;
-constexpr int kKeepOne = 32;
-
 template <typename T, int V, int ACT>
 int run_norm(NormArgs p, int images, bool slab, const Slab& s, hipStream_t stream)
 {
     if (slab)
     {
-        constexpr int kKeep = V == 1 ? kKeepOne : kKeepWide;
+        constexpr int kKeep = keep_of(V);
         p.slab_groups = s.groups;
         p.slabs = (p.groups + s.groups - 1) / s.groups;
         const long long grid = static_cast<long long>(images) * p.slabs;
-        if (grid > INT_MAX)
+        if (grid > INT_MAX - 8)
             return set_error(SV2_EUNSUPPORTED, "sv2_group_norm: too many images");
+        p.blocks = static_cast<int>(grid);
         const void* fn = reinterpret_cast<const void*>(&norm_slab_kernel<T, V, kKeep, ACT>);
         const int rc = set_dynamic_lds(fn, s.lds, "norm_slab: dynamic LDS attribute");
         if (rc != SV2_OK)
             return rc;
-        hipLaunchKernelGGL((norm_slab_kernel<T, V, kKeep, ACT>), dim3(static_cast<unsigned>(grid)), dim3(s.threads),
-                           s.lds, stream, p);
+        hipLaunchKernelGGL((norm_slab_kernel<T, V, kKeep, ACT>), dim3((static_cast<unsigned>(grid) + 7) / 8 * 8),
+                           dim3(s.threads), s.lds, stream, p);
     }
     else
     {
@@ -563,7 +681,8 @@ int run_norm(NormArgs p, int images, bool slab, const Slab& s, hipStream_t strea
         if (rc != SV2_OK)
             return rc;
         hipLaunchKernelGGL((norm_stats_kernel<T, V>), dim3(static_cast<unsigned>(grid)), dim3(kRowThreads), lds, stream, p);
-        hipLaunchKernelGGL(norm_join_kernel, dim3(static_cast<unsigned>(joins)), dim3(64), 0, stream, p);
+        hipLaunchKernelGGL(norm_join_kernel, dim3(static_cast<unsigned>(joins)), dim3(kJoinThreads), 0, stream,
+                           p);
         hipLaunchKernelGGL((norm_apply_kernel<T, V, ACT>), dim3(static_cast<unsigned>(grid)), dim3(kRowThreads), 0, stream, p);
     }
     const hipError_t err = hipGetLastError();
@@ -611,7 +730,7 @@ try
     p.width = channels / groups;
     const int bytes = dtype == SV2_F32 ? 4 : 2;
     // where even single elements fit the slab form, every layout does
-    if (plan_slab(p, 1, kKeepOne, bytes).threads > 0 && plan_slab(p, 16 / bytes, kKeepWide, bytes).threads > 0)
+    if (plan_slab(p, 1, bytes).threads > 0 && plan_slab(p, 16 / bytes, bytes).threads > 0)
         return 0;
     plan_rows(&p, images, bytes);
     return rows_workspace(p, images);
@@ -665,7 +784,7 @@ try
     p.unit = 1;
     while (wide && p.unit < v && p.width % (2 * p.unit) == 0)
         p.unit *= 2;
-    const Slab s = plan_slab(p, wide ? v : 1, wide ? kKeepWide : kKeepOne, bytes);
+    const Slab s = plan_slab(p, wide ? v : 1, bytes);
     const bool slab = s.threads > 0;
     if (!slab)
     {
