@@ -59,7 +59,14 @@
 //                  W halves of a tile are the gate and value rows of the same
 //                  128 columns, Y = fp16(g / (1 + exp(-g)) * u); `rounded`: g
 //                  and u rounded to fp16 first, as the separate products are
+//   kGemmLinear +  the activation's code
+//                  Y = T(act(acc + bias) + R), T fp16 or bf16 (bias, act, R
+//                  optional): sv2_linear's tiles.  Rows of all operands by
+//                  strides, N and K not multiples of the tile: rows of W past
+//                  N repeat the last one and their sums are not stored, and
+//                  the last K % 64 of K go through registers once a tile.
 #include "sv2_internal.h"
+#include "activation.h"
 #include <algorithm>
 #include <climits>
 #include <type_traits>
@@ -90,6 +97,28 @@ constexpr int kPreferRows = 256;    // fewer rows go to the library
 constexpr int kTouchAhead = 3;      // stages before a tile's end
 constexpr float kLog2e = 1.4426950408889634f;
 
+// The 16-bit type of the operands; values are kept as raw 16-bit patterns in
+// the fp16 vector types.
+struct HalfIO
+{
+    static __device__ f4 mfma(h8 a, h8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+    static __device__ float to_float(_Float16 v) { return static_cast<float>(v); }
+    static __device__ _Float16 from_float(float v) { return static_cast<_Float16>(v); }
+};
+struct BfloatIO
+{
+    typedef __attribute__((ext_vector_type(8))) __bf16 b8;
+    static __device__ f4 mfma(h8 a, h8 b, f4 c)
+    {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+    }
+    static __device__ float to_float(_Float16 v)
+    {
+        return __builtin_bit_cast(float, static_cast<unsigned>(__builtin_bit_cast(unsigned short, v)) << 16);
+    }
+    static __device__ _Float16 from_float(float v) { return __builtin_bit_cast(_Float16, static_cast<__bf16>(v)); }
+};
+
 struct TileArgs
 {
     const _Float16* x;  // [M][K]
@@ -105,6 +134,8 @@ struct TileArgs
     int tiles_n;        // column tiles
     int total;          // tiles_m * tiles_n
     int group_m;        // row bands per tile group
+    // kGemmLinear alone
+    long long ldx, ldw, ldy, ldr; // row strides in elements
 };
 
 // Stages an operand tile of MH (X) + NH (W) halves takes, and how many of
@@ -223,10 +254,14 @@ __device__ inline void wait_younger(int n)
 // exponent, below the fp16 roundings of g and u that this form leaves out).
 // Two bodies, not a branch per element: the first costs gate/in at 21658 rows
 // 1166 us where the second takes 1107.
-template <int MH, int NH, int EPI, bool ROUNDED>
+//
+// kGemmLinear: rows by their strides; the columns past N (the last tile's) are
+// left out, a piece that N cuts goes element by element.
+template <int MH, int NH, int EPI, bool ROUNDED, typename IO>
 __device__ __forceinline__ void epilogue(const TileArgs& a, f4 (&acc)[NH][MH][4][2], char* mine, int row0, int col0, int lane)
 {
     constexpr bool kSw = EPI == kGemmSwiGLU;
+    constexpr bool kLin = EPI >= kGemmLinear;
     const int lr = lane & 15;
     const int lq = lane >> 4;
     const int rr = lane >> 3; // rows rr, rr + 8 of the line accesses
@@ -245,6 +280,18 @@ __device__ __forceinline__ void epilogue(const TileArgs& a, f4 (&acc)[NH][MH][4]
         const int col = col0 + kHalf * h;
         f4 gate[4], bias[4];
         u4 res[MH][2][2];
+        const int left = kLin ? a.n - (col + 8 * cc) : 8; // columns of this lane's line piece
+        if constexpr (kLin)
+        {
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                {
+                    const int c = col + 16 * t + 4 * lq + e;
+                    bias[t][e] = a.bias && c < a.n ? a.bias[c] : 0.f;
+                }
+        }
         if constexpr (EPI == kGemmResidual)
         {
 #pragma unroll
@@ -272,11 +319,30 @@ __device__ __forceinline__ void epilogue(const TileArgs& a, f4 (&acc)[NH][MH][4]
 #pragma unroll
         for (int j = 0; j < MH; j++)
         {
+            if (kLin && a.r)
+            {
+#pragma unroll
+                for (int b = 0; b < 2; b++)
+#pragma unroll
+                    for (int s = 0; s < 2; s++)
+                    {
+                        const int row = min(row0 + kHalf * j + 16 * b + rr + 8 * s, a.m - 1);
+                        const _Float16* from = a.r + row * a.ldr + col + 8 * cc;
+                        h8 v = {};
+                        if (left >= 8)
+                            v = __builtin_bit_cast(h8, __builtin_nontemporal_load(reinterpret_cast<const u4*>(from)));
+                        else
+#pragma unroll
+                            for (int e = 0; e < 8; e++) // the columns past N: anything that may be read
+                                v[e] = a.r[row * a.ldr + min(col + 8 * cc + e, a.n - 1)];
+                        res[j][b][s] = __builtin_bit_cast(u4, v);
+                    }
+            }
 #pragma unroll
             for (int b = 0; b < 2; b++)
             {
                 h4 old[4];
-                if constexpr (EPI == kGemmResidual)
+                if (EPI == kGemmResidual || (kLin && a.r))
                 {
                     *reinterpret_cast<u4*>(line[0]) = res[j][b][0];
                     *reinterpret_cast<u4*>(line[1]) = res[j][b][1];
@@ -327,7 +393,13 @@ __device__ __forceinline__ void epilogue(const TileArgs& a, f4 (&acc)[NH][MH][4]
                                 v = v + r;
                             }
                         }
-                        o[e] = static_cast<_Float16>(v);
+                        if constexpr (kLin)
+                        {
+                            v = activate<EPI - kGemmLinear, false>(v + bias[t][e]);
+                            if (a.r)
+                                v += IO::to_float(old[t][e]);
+                        }
+                        o[e] = IO::from_float(v);
                     }
                     *reinterpret_cast<h4*>(quad[t]) = o;
                 }
@@ -337,7 +409,17 @@ __device__ __forceinline__ void epilogue(const TileArgs& a, f4 (&acc)[NH][MH][4]
                 {
                     const int row = row0 + kHalf * j + 16 * b + rr + 8 * s;
                     const u4 v = *reinterpret_cast<const u4*>(line[s]);
-                    if (row < a.m)
+                    if constexpr (kLin)
+                    {
+                        _Float16* to = a.y + row * a.ldy + col + 8 * cc;
+                        if (row < a.m && left >= 8)
+                            __builtin_nontemporal_store(v, reinterpret_cast<u4*>(to));
+                        else if (row < a.m)
+#pragma nounroll
+                            for (int e = 0; e < left; e++)
+                                to[e] = reinterpret_cast<const _Float16*>(line[s])[e];
+                    }
+                    else if (row < a.m)
                         __builtin_nontemporal_store(v, reinterpret_cast<u4*>(a.y + static_cast<long long>(row) * a.n + col + 8 * cc));
                 }
                 lds_order();
@@ -346,11 +428,12 @@ __device__ __forceinline__ void epilogue(const TileArgs& a, f4 (&acc)[NH][MH][4]
     }
 }
 
-template <int MH, int NH, int EPI, bool KS>
+template <int MH, int NH, int EPI, bool KS, typename IO>
 __global__ __launch_bounds__(kThreads) void gemm_tile_kernel(TileArgs a)
 {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     using S = Shape<MH, NH>;
+    constexpr bool kLin = EPI >= kGemmLinear;
     constexpr int kSlots = S::kSlots;
     constexpr int kFour = MH == 2 && NH == 2; // four phases a stage
     static_assert(!KS || MH + NH == 2, "the K-split form is the 128 x 128 one");
@@ -367,7 +450,8 @@ __global__ __launch_bounds__(kThreads) void gemm_tile_kernel(TileArgs a)
     const int lr = lane & 15;
     const int lq = lane >> 4;
     const int nk = a.k / kBK;
-    const unsigned k2 = 2u * static_cast<unsigned>(a.k);
+    const unsigned k2 = 2u * static_cast<unsigned>(kLin ? a.ldx : a.k); // bytes between rows of X
+    const unsigned w2 = kLin ? 2u * static_cast<unsigned>(a.ldw) : k2;    // and of W
 
     // tile list of this workgroup: round r gives XCD x the contiguous ids
     // [r G + x G/8, + G/8), the last round an even share of what is left
@@ -398,6 +482,7 @@ __global__ __launch_bounds__(kThreads) void gemm_tile_kernel(TileArgs a)
     const unsigned chunk0 = 16u * ((lane & 7) ^ (lane >> 4));
     const unsigned vw0 = frow * k2 + chunk0;
     const unsigned vw1 = (frow + 8) * k2 + (chunk0 ^ 64u);
+    unsigned vw[NH][2]; // kGemmLinear: by tile
     unsigned vx[MH][2];
     const char* fx = nullptr;       // X rows of the tile being fetched, at the stage being fetched
     const char* fw[NH];
@@ -423,6 +508,16 @@ __global__ __launch_bounds__(kThreads) void gemm_tile_kernel(TileArgs a)
         {
             const _Float16* src = (EPI == kGemmSwiGLU && h == 1) ? a.w2 : a.w;
             const int row = (EPI == kGemmSwiGLU) ? n0 : n0 + kHalf * h;
+            if constexpr (kLin)
+            {
+                // rows past N repeat the last one; their sums are never stored
+                const int first = min(row, a.n - 1);
+                const int lastw = a.n - 1 - first;
+                vw[h][0] = static_cast<unsigned>(min(static_cast<int>(frow), lastw)) * w2 + chunk0;
+                vw[h][1] = static_cast<unsigned>(min(static_cast<int>(frow + 8), lastw)) * w2 + (chunk0 ^ 64u);
+                fw[h] = reinterpret_cast<const char*>(src) + static_cast<unsigned long long>(first) * w2;
+                continue;
+            }
             fw[h] = reinterpret_cast<const char*>(src) + static_cast<unsigned long long>(row) * k2;
         }
     };
@@ -430,8 +525,8 @@ __global__ __launch_bounds__(kThreads) void gemm_tile_kernel(TileArgs a)
     const unsigned lds_wave = lds0 + 16u * wave * kRowBytes;
     auto fetch_w = [&](int h) {
         const unsigned d = lds_wave + f_slot + h * kHalfBytes;
-        dma16(fw[h], vw0, d);
-        dma16(fw[h], vw1, d + 8 * kRowBytes);
+        dma16(fw[h], kLin ? vw[h][0] : vw0, d);
+        dma16(fw[h], kLin ? vw[h][1] : vw1, d + 8 * kRowBytes);
     };
     auto fetch_x = [&](int j) {
         const unsigned d = lds_wave + f_slot + (NH + j) * kHalfBytes;
@@ -488,8 +583,7 @@ __global__ __launch_bounds__(kThreads) void gemm_tile_kernel(TileArgs a)
             for (int t = 0; t < 4; t++)
 #pragma unroll
                 for (int b = 0; b < kXT; b++)
-                    acc[h][j][t][b] =
-                        __builtin_amdgcn_mfma_f32_16x16x32_f16(rw[ks][t], rx[j][ks][b], acc[h][j][t][b], 0, 0, 0);
+                    acc[h][j][t][b] = IO::mfma(rw[ks][t], rx[j][ks][b], acc[h][j][t][b]);
     };
 
     auto read_slot_next = [&]() {
@@ -685,6 +779,45 @@ __global__ __launch_bounds__(kThreads) void gemm_tile_kernel(TileArgs a)
         for (; i < nk; i++)
             stage(std::false_type{}, g++);
         char* mine = smem + kSlots * S::kStageBytes + wave * kEpiWave;
+        if constexpr (kLin)
+        {
+            // the last K % 64, 32 at a time (KS: each group's own step)
+            for (int k0 = nk * kBK + (KS ? 32 * grp : 0); k0 < a.k; k0 += KS ? kBK : 32)
+            {
+                const int kc = k0 + 8 * lq; // a multiple of 8, as K's pieces are
+                auto piece = [&](const _Float16* row) {
+                    h8 v = {};
+                    if (kc + 8 <= a.k)
+                        v = *reinterpret_cast<const h8*>(row + kc);
+                    else
+#pragma unroll
+                        for (int e = 0; e < 8; e++) // branch-free: this stands 16 times in a tile
+                        {
+                            const _Float16 x = row[min(kc + e, a.k - 1)];
+                            v[e] = kc + e < a.k ? x : static_cast<_Float16>(0.f);
+                        }
+                    return v;
+                };
+#pragma unroll
+                for (int h = 0; h < NH; h++)
+                {
+                    h8 tw[4];
+#pragma unroll
+                    for (int t = 0; t < 4; t++)
+                        tw[t] = piece(a.w + min(n0 + kHalf * h + wrow + 16 * t + lr, a.n - 1) * a.ldw);
+#pragma unroll
+                    for (int j = 0; j < MH; j++)
+#pragma unroll
+                        for (int b = 0; b < kXT; b++)
+                        {
+                            const h8 tx = piece(a.x + min(m0 + kHalf * j + xrow + 16 * b + lr, a.m - 1) * a.ldx);
+#pragma unroll
+                            for (int t = 0; t < 4; t++)
+                                acc[h][j][t][b] = IO::mfma(tw[t], tx, acc[h][j][t][b]);
+                        }
+                }
+            }
+        }
         if constexpr (KS)
         {
             // one tile per workgroup: the stage slots are free once both
@@ -711,15 +844,15 @@ __global__ __launch_bounds__(kThreads) void gemm_tile_kernel(TileArgs a)
 #pragma unroll
                 for (int b = 0; b < 2; b++)
                     sum[0][0][t][b] += take[(2 * t + b) * 64];
-            epilogue<1, 1, EPI, false>(a, sum, mine, m0 + xrow + 32 * grp, n0 + wrow, lane);
+            epilogue<1, 1, EPI, false, IO>(a, sum, mine, m0 + xrow + 32 * grp, n0 + wrow, lane);
             return;
         }
         else
         {
             if (EPI == kGemmSwiGLU && a.rounded)
-                epilogue<MH, NH, EPI, true>(a, acc, mine, m0 + xrow, n0 + wrow, lane);
+                epilogue<MH, NH, EPI, true, IO>(a, acc, mine, m0 + xrow, n0 + wrow, lane);
             else
-                epilogue<MH, NH, EPI, false>(a, acc, mine, m0 + xrow, n0 + wrow, lane);
+                epilogue<MH, NH, EPI, false, IO>(a, acc, mine, m0 + xrow, n0 + wrow, lane);
             clear();
         }
     }
@@ -727,19 +860,19 @@ __global__ __launch_bounds__(kThreads) void gemm_tile_kernel(TileArgs a)
         bar();
 }
 
-template <int MH, int NH, int EPI, bool KS = false>
+template <int MH, int NH, int EPI, bool KS = false, typename IO = HalfIO>
 int launch(const TileArgs& a, hipStream_t stream)
 {
     using S = Shape<MH, NH>;
-    const void* fn = reinterpret_cast<const void*>(&gemm_tile_kernel<MH, NH, EPI, KS>);
+    const void* fn = reinterpret_cast<const void*>(&gemm_tile_kernel<MH, NH, EPI, KS, IO>);
     const int rc = set_dynamic_lds(fn, S::kLds, "gemm_f16: dynamic LDS attribute");
     if (rc != SV2_OK)
         return rc;
     // a multiple of the 8 XCDs; KS: one tile per workgroup
     const int all = (a.total + 7) / 8 * 8;
     const int grid = KS ? all : std::min(kCus, all);
-    hipLaunchKernelGGL((gemm_tile_kernel<MH, NH, EPI, KS>), dim3(static_cast<unsigned>(grid)), dim3(kThreads), S::kLds,
-                       stream, a);
+    hipLaunchKernelGGL((gemm_tile_kernel<MH, NH, EPI, KS, IO>), dim3(static_cast<unsigned>(grid)), dim3(kThreads),
+                       S::kLds, stream, a);
     const hipError_t err = hipGetLastError();
     return err == hipSuccess ? SV2_OK : hip_error(err, "gemm_tile_kernel launch");
 }
@@ -769,7 +902,8 @@ constexpr double kLaunch = 7.0; // launch, first fetches, drain
 
 long long tiles_of(Form f, int rows, long long wrows)
 {
-    return (static_cast<long long>(rows) + kCost[f].rows - 1) / kCost[f].rows * (wrows / kCost[f].cols);
+    return (static_cast<long long>(rows) + kCost[f].rows - 1) / kCost[f].rows *
+           ((wrows + kCost[f].cols - 1) / kCost[f].cols);
 }
 
 double form_us(Form f, int rows, int in, long long wrows)
@@ -822,7 +956,7 @@ Plan make_plan(int rows, int in, int out, int epi, bool rounded)
         if (us < best.us)
             best = Plan{0, forms[i], us};
     }
-    const long long per_band = wrows / 256;
+    const long long per_band = (wrows + 255) / 256;
     const long long bands = static_cast<long long>(kCus) * (tiles_of(kBig, rows, wrows) / kCus) / per_band;
     const long long first = bands * 256;
     if (first > 0 && first < rows)
@@ -877,6 +1011,43 @@ int run_rows(Form f, TileArgs a, int epi, int r0, int rows, hipStream_t stream)
     case kGemmStore: return launch_form<kGemmStore>(f, a, stream);
     case kGemmResidual: return launch_form<kGemmResidual>(f, a, stream);
     default: return launch_form<kGemmSwiGLU>(f, a, stream);
+    }
+}
+
+template <int ACT>
+int launch_linear(Form f, const TileArgs& a, bool bf16, hipStream_t stream)
+{
+    constexpr int kEpi = kGemmLinear + ACT;
+    switch (f)
+    {
+    case kBig: return bf16 ? launch<2, 2, kEpi, false, BfloatIO>(a, stream) : launch<2, 2, kEpi>(a, stream);
+    case kTall: return bf16 ? launch<2, 1, kEpi, false, BfloatIO>(a, stream) : launch<2, 1, kEpi>(a, stream);
+    case kSmall: return bf16 ? launch<1, 1, kEpi, false, BfloatIO>(a, stream) : launch<1, 1, kEpi>(a, stream);
+    default: return bf16 ? launch<1, 1, kEpi, true, BfloatIO>(a, stream) : launch<1, 1, kEpi, true>(a, stream);
+    }
+}
+
+// sv2_linear's rows r0 .. r0 + rows in form f.
+int run_linear_rows(Form f, TileArgs a, int act, bool bf16, int r0, int rows, hipStream_t stream)
+{
+    a.x += r0 * a.ldx;
+    a.y += r0 * a.ldy;
+    if (a.r)
+        a.r += r0 * a.ldr;
+    a.m = rows;
+    a.tiles_m = (rows + kCost[f].rows - 1) / kCost[f].rows;
+    a.tiles_n = (a.n + kCost[f].cols - 1) / kCost[f].cols;
+    const long long total = tiles_of(f, rows, a.n);
+    if (total > INT_MAX - kCus)
+        return set_error(SV2_EUNSUPPORTED, "linear: too many tiles");
+    a.total = static_cast<int>(total);
+    a.group_m = 8;
+    switch (act)
+    {
+    case SV2_ACT_SILU: return launch_linear<SV2_ACT_SILU>(f, a, bf16, stream);
+    case SV2_ACT_GELU: return launch_linear<SV2_ACT_GELU>(f, a, bf16, stream);
+    case SV2_ACT_GELU_TANH: return launch_linear<SV2_ACT_GELU_TANH>(f, a, bf16, stream);
+    default: return launch_linear<SV2_ACT_NONE>(f, a, bf16, stream);
     }
 }
 
@@ -1015,6 +1186,38 @@ int gemm_mfma(hipStream_t stream, int rows, int in, int out, const void* x, cons
             return rc;
     }
     return run_rows(plan.rest, a, epi, plan.first_rows, rows - plan.first_rows, stream);
+}
+
+bool linear_tiles_fit(const LinearOperands& o)
+{
+    // a tile's rows are addressed by 32-bit offsets from its first
+    constexpr long long kMostStride = (1LL << 31) / (2 * 256);
+    return o.k >= kBK && o.ldx % 8 == 0 && o.ldw % 8 == 0 && o.ldy % 8 == 0 && o.ldr % 8 == 0 && o.ldx < kMostStride &&
+           o.ldw < kMostStride && !misaligned(o.x, 16) && !misaligned(o.w, 16) && !misaligned(o.y, 16) && !misaligned(o.r, 16);
+}
+
+int linear_tiles(hipStream_t stream, const LinearOperands& o)
+{
+    TileArgs a{};
+    a.x = static_cast<const _Float16*>(o.x);
+    a.w = static_cast<const _Float16*>(o.w);
+    a.y = static_cast<_Float16*>(o.y);
+    a.r = static_cast<const _Float16*>(o.r);
+    a.bias = o.bias;
+    a.n = o.n;
+    a.k = o.k;
+    a.ldx = o.ldx;
+    a.ldw = o.ldw;
+    a.ldy = o.ldy;
+    a.ldr = o.ldr;
+    const Plan plan = make_plan(o.m, o.k, o.n, kGemmLinear, false);
+    if (plan.first_rows > 0)
+    {
+        const int rc = run_linear_rows(kBig, a, o.act, o.bf16, 0, plan.first_rows, stream);
+        if (rc != SV2_OK)
+            return rc;
+    }
+    return run_linear_rows(plan.rest, a, o.act, o.bf16, plan.first_rows, o.m - plan.first_rows, stream);
 }
 
 } // namespace sv2

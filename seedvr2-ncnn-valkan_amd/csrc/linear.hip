@@ -512,6 +512,9 @@ try
             return whole ? run_few_rows<HalfIO, true>(p, st) : run_few_rows<HalfIO, false>(p, st);
         return whole ? run_few_rows<BfloatIO, true>(p, st) : run_few_rows<BfloatIO, false>(p, st);
     }
+    const LinearOperands o{p.x, p.w, p.y, p.r, p.bias, p.ldx, p.ldw, p.ldy, p.ldr, p.m, p.n, p.k, p.act, a.dtype == SV2_BF16};
+    if (linear_tiles_fit(o))
+        return linear_tiles(st, o);
     return a.dtype == SV2_F16 ? run_act<HalfIO>(p, a.activation, st) : run_act<BfloatIO>(p, a.activation, st);
 }
 catch (...)

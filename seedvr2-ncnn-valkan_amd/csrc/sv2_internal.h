@@ -199,6 +199,26 @@ bool gemm_mfma_preferred(int rows, int in, int out, int epi, const void* x, cons
 int gemm_mfma(hipStream_t stream, int rows, int in, int out, const void* x, const void* w, const void* w2, void* y,
               int epi, bool rounded, const float* bias, const float* gate, const void* residual);
 
+// The operands of sv2_linear: y = act(x W^T + bias) + r, strides in elements,
+// r and bias may be null.
+struct LinearOperands
+{
+    const void* x;
+    const void* w;
+    void* y;
+    const void* r;
+    const float* bias;
+    long long ldx, ldw, ldy, ldr;
+    int m, n, k;
+    int act;  // sv2_activation
+    bool bf16; // else fp16
+};
+// The product on gemm_mfma's tiles, and whether they take these operands
+// (16-byte aligned, strides a multiple of 8 elements, k >= 64).
+constexpr int kGemmLinear = 3; // + sv2_activation: the tile kernel's epilogue codes from here on
+bool linear_tiles_fit(const LinearOperands& o);
+int linear_tiles(hipStream_t stream, const LinearOperands& o);
+
 // fp16 y = epilogue(x W^T) for 1-64 rows on the weight-streaming kernel
 // (gemm_few.hip), the same epilogues as gemm_mfma (kGemmStore also takes an
 // optional bias: y = fp16(fp16(x W^T) + bias)).  Needs in % 64 == 0 and
