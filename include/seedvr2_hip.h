@@ -640,8 +640,8 @@ typedef struct sv2_sliding_attn_args {
 int64_t sv2_sliding_attention_workspace(const sv2_sliding_attn_args* args);
 
 /* Device.  The attention above.  q, k, v, out and the workspace must be
- * 16-byte aligned and every stride a multiple of 8 elements (SV2_EINVAL);
- * token strides of k and v up to 2^24 elements, head_dim 64 or 128
+ * 16-byte aligned and every stride a multiple of 8 elements (SV2_EINVAL; the
+ * stride of a dimension of one element is not read); token strides of k and v up to 2^24 elements, head_dim 64 or 128
  * (SV2_EUNSUPPORTED).  Results do not depend on timing. */
 int sv2_sliding_attention(const sv2_sliding_attn_args* args, void* stream);
 

@@ -95,7 +95,7 @@ struct SlideParams
     float scale2;   // scale * log2(e)
     int batch, q_len, kv_len, heads, kv_heads, group;
     int left, right, sinks;
-    int row_tiles, splits, blocks;
+    int few, row_tiles, splits, blocks;
 };
 
 constexpr int kKeys = 64;      // keys of a tile
@@ -174,30 +174,29 @@ __device__ inline u2 keys4(const char* at)
     return __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at)));
 }
 
-// The keys a tile of rows at positions p0 .. p1 visits: tiles of the first
-// tokens, then those of the window.
+// The keys that rows at positions p0 .. p1 visit, in tiles of KEYS: those of
+// the first tokens, then those of the window.
+template <int KEYS>
 struct KeyTiles
 {
     int sink, start, count;
-    __device__ int at(int i) const { return i < sink ? i : start + i - sink; }
+    __device__ KeyTiles(const SlideParams& p, int nk, int p0, int p1) : sink(0), start(0), count(0)
+    {
+        const int hi = min(nk, p1 + p.right + 1); // one past the last visible key
+        if (hi <= 0)
+            return;
+        sink = (min(p.sinks, hi) + KEYS - 1) / KEYS;
+        start = max(max(0, p0 - p.left) / KEYS, sink);
+        count = sink + max(0, (hi + KEYS - 1) / KEYS - start);
+    }
+    // first key of tile i
+    __device__ int key(int i) const { return (i < sink ? i : start + i - sink) * KEYS; }
 };
-__device__ inline KeyTiles key_tiles(const SlideParams& p, int nk, int p0, int p1)
-{
-    const int hi = min(nk, p1 + p.right + 1); // one past the last visible key
-    KeyTiles t{0, 0, 0};
-    if (hi <= 0)
-        return t;
-    const int lo = max(0, p0 - p.left);
-    t.sink = (min(p.sinks, hi) + kKeys - 1) / kKeys;
-    t.start = max(lo / kKeys, t.sink);
-    t.count = t.sink + max(0, (hi + kKeys - 1) / kKeys - t.start);
-    return t;
-}
 
-// LDS of one tile: keys, then values, rows of D elements.  16-byte chunk c of
-// row r sits in slot c ^ key_swz(r) (the 16 rows that an operand read takes
-// fall on different bank groups) or c ^ value_swz(r) (the four rows of a
-// transposing read do).
+// LDS tiles of keys and values: rows of D elements, 16-byte chunk c of row r
+// in slot c ^ key_swz(r) (the 16 rows that an operand read takes fall on
+// different bank groups) or c ^ value_swz(r) (the four rows of a transposing
+// read do).
 template <int D>
 __device__ inline unsigned key_swz(unsigned r)
 {
@@ -209,159 +208,110 @@ __device__ inline unsigned value_swz(unsigned r)
     return D == 128 ? (r & 3) << 2 : ((r >> 1) & 1) << 2;
 }
 
+// 32 query rows in one wave: lane % 32 is the row (its two half-waves hold
+// different keys of the scores and different dims of the sums).
 template <typename IO, int D>
-__global__ __launch_bounds__(64 * kWaves, 2) void slide_tile_kernel(SlideParams p)
+struct Rows
 {
-    extern __shared__ __attribute__((aligned(16))) char smem[];
-    constexpr int kRowBytes = 2 * D;
-    constexpr int kChunks = kRowBytes / 16;
-    constexpr int kTileBytes = kKeys * kRowBytes;
-    constexpr int kBuf = 2 * kTileBytes;
-    constexpr int kSteps = D / 16;
-    constexpr int kBlocks = D / 32;
-    constexpr int kRowsPerDma = 64 / kChunks;
-    constexpr int kDma = kKeys / kRowsPerDma / kWaves; // of each of K and V per wave
-
-    // XCD x (workgroup id mod 8) takes a contiguous run of blocks: tiles of one
-    // key head share an L2
-    const int per = gridDim.x >> 3;
-    const int id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-    if (id >= p.blocks)
-        return;
-    const int tile = id % p.row_tiles;
-    int rest = id / p.row_tiles;
-    const int split = rest % p.splits;
-    rest /= p.splits;
-    const int kvh = rest % p.kv_heads;
-    const int b = rest / p.kv_heads;
-
-    const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int half = lane >> 5;
-    const int nq = __builtin_amdgcn_readfirstlane(clamp_len(p.q_lens, b, p.q_len));
-    const int nk = __builtin_amdgcn_readfirstlane(clamp_len(p.kv_lens, b, p.kv_len));
-    const int rows = nq * p.group;
-    const int first = tile * kRows;
-    if (first >= rows)
-        return;
-    const int off = nk - nq;
-    const int p0 = off + first / p.group;
-    const int p1 = off + (min(first + kRows, rows) - 1) / p.group;
-    const KeyTiles kt = key_tiles(p, nk, p0, p1);
-    const int share = (kt.count + p.splits - 1) / p.splits;
-    const int t0 = min(split * share, kt.count);
-    const int t1 = min(t0 + share, kt.count);
-
-    const int row = first + wave * 32 + (lane & 31);
-    const bool live = row < rows;
-    const int rowc = min(row, rows - 1);
-    const int qi = rowc / p.group;
-    const int head = kvh * p.group + (rowc - qi * p.group);
-    const int pos = off + qi;
-    const int hi_key = min(pos + p.right, nk - 1);
-    const int lo_key = pos - p.left;
+    static constexpr int kRowBytes = 2 * D;
+    static constexpr int kSteps = D / 16;
+    static constexpr int kBlocks = D / 32;
 
     u4 q[kSteps];
+    f16v o[kBlocks]; // sums, dims 32 i + 8 (e / 4) + 4 half + e % 4
+    float m;         // largest score so far, times scale2
+    float l;         // this half-wave's part of the sum of weights
+    int half, qi, head, hi_key, lo_key, sinks;
+    float scale2;
+    unsigned koff[kSteps], voff[kBlocks];
+
+    // row `row` (a packed one, clamped by the caller) of key head kvh, the
+    // sequence's first query at position `off`
+    __device__ void init(const SlideParams& p, int b, int kvh, int row, int off, int nk, int lane)
     {
+        half = lane >> 5;
+        qi = row / p.group;
+        head = kvh * p.group + (row - qi * p.group);
+        hi_key = min(off + qi + p.right, nk - 1);
+        lo_key = off + qi - p.left;
+        sinks = p.sinks;
+        scale2 = p.scale2;
         const char* qr = p.q + b * p.q_b + qi * p.q_t + head * p.q_h + 16 * half;
 #pragma unroll
-        for (int s = 0; s < kSteps; s++)
-            q[s] = *reinterpret_cast<const u4*>(qr + 32 * s);
-    }
-
-    const char* kb = p.k + b * p.k_b + kvh * p.k_h;
-    const char* vb = p.v + b * p.v_b + kvh * p.v_h;
-    const unsigned lds0 = static_cast<unsigned>(reinterpret_cast<size_t>(smem));
-    const unsigned k_step = static_cast<unsigned>(p.k_t);
-    const unsigned v_step = static_cast<unsigned>(p.v_t);
-    auto fetch = [&](int t, int buf) {
-        const int k0 = t * kKeys;
-        const int last = nk - 1 - k0; // rows past the end repeat the last one
-        const char* kp = kb + k0 * p.k_t;
-        const char* vp = vb + k0 * p.v_t;
-        const unsigned d = lds0 + buf * kBuf;
+        for (int c = 0; c < kSteps; c++)
+            q[c] = *reinterpret_cast<const u4*>(qr + 32 * c);
 #pragma unroll
-        for (int i = 0; i < kDma; i++)
+        for (int i = 0; i < kBlocks; i++)
+#pragma unroll
+            for (int e = 0; e < 16; e++)
+                o[i][e] = 0.f;
+        m = kNegInf;
+        l = 0.f;
+        const unsigned krow = lane & 31;
+#pragma unroll
+        for (int c = 0; c < kSteps; c++)
+            koff[c] = krow * kRowBytes + (((2 * c + half) ^ key_swz<D>(krow)) << 4);
+        // transposing reads: rows 4 half + (lane % 16) / 4 of a group of 8 keys,
+        // dims 32 i + 16 (lane / 16 % 2) + 4 (lane % 4)
+        const unsigned vrow = 4 * half + ((lane & 15) >> 2);
+#pragma unroll
+        for (int i = 0; i < kBlocks; i++)
         {
-            const int r0 = (wave * kDma + i) * kRowsPerDma;
-            const unsigned r = r0 + lane / kChunks;
-            const unsigned c = lane % kChunks;
-            const unsigned rr = min(static_cast<int>(r), last);
-            dma16(kp, rr * k_step + ((c ^ key_swz<D>(r)) << 4), d + r0 * kRowBytes);
-            dma16(vp, rr * v_step + ((c ^ value_swz<D>(r)) << 4), d + kTileBytes + r0 * kRowBytes);
+            const unsigned c = 4 * i + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+            voff[i] = vrow * kRowBytes + ((c ^ value_swz<D>(vrow)) << 4) + 8 * (lane & 1);
         }
-    };
-
-    f16v o[kBlocks];
-#pragma unroll
-    for (int i = 0; i < kBlocks; i++)
-#pragma unroll
-        for (int e = 0; e < 16; e++)
-            o[i][e] = 0.f;
-    float m = kNegInf; // largest score so far, times scale2
-    float l = 0.f;     // this half-wave's part of the sum of weights
-
-    // operand reads
-    const unsigned krow = lane & 31;
-    unsigned koff[kSteps];
-#pragma unroll
-    for (int s = 0; s < kSteps; s++)
-        koff[s] = krow * kRowBytes + (((2 * s + half) ^ key_swz<D>(krow)) << 4);
-    // transposing reads: rows 4 half + (lane % 16) / 4 of a group of 8 keys,
-    // dims 32 blk + 16 (lane / 16 % 2) + 4 (lane % 4)
-    const unsigned vrow = 4 * half + ((lane & 15) >> 2);
-    unsigned voff[kBlocks];
-#pragma unroll
-    for (int i = 0; i < kBlocks; i++)
-    {
-        const unsigned c = 4 * i + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-        voff[i] = kTileBytes + vrow * kRowBytes + ((c ^ value_swz<D>(vrow)) << 4) + 8 * (lane & 1);
     }
+    // key of score e of key block i of a tile from key k0 on
+    __device__ int key_of(int k0, int i, int e) const { return k0 + 4 * half + 32 * i + 8 * (e >> 2) + (e & 3); }
+    __device__ bool sees(int j) const { return (j <= hi_key) & ((j < sinks) | (j >= lo_key)); }
 
-    if (t0 < t1)
+    template <int NB>
+    __device__ void scores(f16v (&s)[NB], const char* keys) const
     {
-        fetch(kt.at(t0), 0);
-    }
-    for (int t = t0; t < t1; t++)
-    {
-        const int buf = (t - t0) & 1;
-        wait_vm<0>();
-        bar(); // the tile is whole, and the other buffer's readers are done
-        if (t + 1 < t1)
-            fetch(kt.at(t + 1), buf ^ 1);
-        const int k0 = kt.at(t) * kKeys;
-        const char* st = smem + buf * kBuf;
-        f16v s[2];
 #pragma unroll
-        for (int i = 0; i < 2; i++)
+        for (int i = 0; i < NB; i++)
         {
 #pragma unroll
             for (int e = 0; e < 16; e++)
                 s[i][e] = 0.f;
 #pragma unroll
             for (int c = 0; c < kSteps; c++)
-                s[i] = IO::mfma(*reinterpret_cast<const u4*>(st + i * 32 * kRowBytes + koff[c]), q[c], s[i]);
+                s[i] = IO::mfma(*reinterpret_cast<const u4*>(keys + i * 32 * kRowBytes + koff[c]), q[c], s[i]);
         }
-        const bool masked = !(k0 + kKeys <= nk && k0 + kKeys - 1 <= p0 + p.right &&
-                              (k0 + kKeys <= p.sinks || k0 >= p1 - p.left));
-        auto key_of = [&](int i, int e) { return k0 + 32 * i + 8 * (e >> 2) + 4 * half + (e & 3); };
-        auto sees = [&](int j) { return j <= hi_key && (j < p.sinks || j >= lo_key); };
-        if (masked)
+    }
+    template <int NB>
+    __device__ void mask(f16v (&s)[NB], int k0) const
+    {
+        if (k0 >= sinks)
         {
+            // lo_key <= j <= hi_key in one comparison (hi_key < lo_key: nothing)
+            const unsigned range = hi_key >= lo_key ? static_cast<unsigned>(hi_key - lo_key) : 0u;
+            const int d = hi_key >= lo_key ? k0 - lo_key : -(1 << 30);
 #pragma unroll
-            for (int i = 0; i < 2; i++)
+            for (int i = 0; i < NB; i++)
 #pragma unroll
                 for (int e = 0; e < 16; e++)
-                    s[i][e] = sees(key_of(i, e)) ? s[i][e] : kNegInf;
+                    s[i][e] = static_cast<unsigned>(key_of(d, i, e)) <= range ? s[i][e] : kNegInf;
+            return;
         }
+#pragma unroll
+        for (int i = 0; i < NB; i++)
+#pragma unroll
+            for (int e = 0; e < 16; e++)
+                s[i][e] = sees(key_of(k0, i, e)) ? s[i][e] : kNegInf;
+    }
+    // scores to weights exp2(s scale2 - m), rounded for the product; the sums
+    // so far are rescaled when some row's maximum rose
+    template <int NB>
+    __device__ void weights(f16v (&s)[NB], u4 (&w)[2 * NB])
+    {
         float top = kNegInf;
 #pragma unroll
-        for (int i = 0; i < 2; i++)
+        for (int i = 0; i < NB; i++)
 #pragma unroll
             for (int e = 0; e < 16; e++)
                 top = fmaxf(top, s[i][e]);
-        top = partner_max(top) * p.scale2;
-        // the sums are rescaled only when some row's maximum rose
+        top = partner_max(top) * scale2;
         if (__builtin_amdgcn_ballot_w64(top > m) != 0)
         {
             const float next = fmaxf(top, m);
@@ -376,138 +326,439 @@ __global__ __launch_bounds__(64 * kWaves, 2) void slide_tile_kernel(SlideParams 
         }
         const float base = m == kNegInf ? 0.f : m;
 #pragma unroll
-        for (int i = 0; i < 2; i++)
+        for (int i = 0; i < NB; i++)
 #pragma unroll
             for (int e = 0; e < 16; e++)
             {
-                s[i][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][e], p.scale2, -base));
+                s[i][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][e], scale2, -base));
                 l += s[i][e];
             }
-        u4 w[4];
 #pragma unroll
-        for (int c = 0; c < 4; c++)
+        for (int c = 0; c < 2 * NB; c++)
 #pragma unroll
             for (int e = 0; e < 4; e++)
                 w[c][e] = IO::pack(s[c >> 1][8 * (c & 1) + 2 * e], s[c >> 1][8 * (c & 1) + 2 * e + 1]);
+    }
+    // values of keys 16 c .. 16 c + 15 of a tile, dims 32 i on
+    __device__ u4 values(const char* vals, int i, int c) const
+    {
+        const u2 lo = keys4(vals + voff[i] + 16 * c * kRowBytes);
+        const u2 hi = keys4(vals + voff[i] + (16 * c + 8) * kRowBytes);
+        return u4{lo.x, lo.y, hi.x, hi.y};
+    }
+    // sums += weights values; in a masked tile (from key k0 on) values that
+    // are not finite stay out of the product
+    template <int NB>
+    __device__ void add(const u4 (&w)[2 * NB], const char* vals, int k0, bool masked)
+    {
 #pragma unroll
         for (int i = 0; i < kBlocks; i++)
         {
-            u4 a[4];
+            u4 a[2 * NB];
 #pragma unroll
-            for (int c = 0; c < 4; c++)
-            {
-                const u2 lo = keys4(st + voff[i] + 16 * c * kRowBytes);
-                const u2 hi = keys4(st + voff[i] + (16 * c + 8) * kRowBytes);
-                a[c] = u4{lo.x, lo.y, hi.x, hi.y};
-            }
+            for (int c = 0; c < 2 * NB; c++)
+                a[c] = values(vals, i, c);
             if (masked)
             {
                 unsigned bad = 0;
 #pragma unroll
-                for (int c = 0; c < 4; c++)
+                for (int c = 0; c < 2 * NB; c++)
 #pragma unroll
                     for (int e = 0; e < 4; e++)
                         bad |= (a[c][e] & IO::kExpMask) + IO::kExpOne;
-                if (__builtin_amdgcn_ballot_w64((bad & 0x80008000u) != 0) != 0)
-                {
-                    // the sums of visible values that are +Inf, -Inf or NaN,
-                    // by counting them
-                    u4 vis[4];
-#pragma unroll
-                    for (int c = 0; c < 4; c++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-                        {
-                            const int at = 8 * (c & 1) + 2 * e;
-                            vis[c][e] = (sees(key_of(c >> 1, at)) ? IO::kOne : 0u) |
-                                        (sees(key_of(c >> 1, at + 1)) ? IO::kOne << 16 : 0u);
-                        }
-                    const unsigned inf = IO::kExpMask & 0xffffu;
-#pragma unroll
-                    for (int kind = 0; kind < 3; kind++)
-                    {
-                        f16v n;
-#pragma unroll
-                        for (int e = 0; e < 16; e++)
-                            n[e] = 0.f;
-#pragma unroll
-                        for (int c = 0; c < 4; c++)
-                        {
-                            u4 is;
-#pragma unroll
-                            for (int e = 0; e < 4; e++)
-                            {
-                                auto flag = [&](unsigned x) {
-                                    const bool hit = kind == 0   ? x == inf
-                                                     : kind == 1 ? x == (inf | 0x8000u)
-                                                                 : (x & 0x7fffu) > inf;
-                                    return hit ? IO::kOne : 0u;
-                                };
-                                is[e] = flag(a[c][e] & 0xffffu) | flag(a[c][e] >> 16) << 16;
-                            }
-                            n = IO::mfma(is, vis[c], n);
-                        }
-                        const float add = kind == 0 ? -kNegInf : kind == 1 ? kNegInf : __builtin_nanf("");
-#pragma unroll
-                        for (int e = 0; e < 16; e++)
-                            o[i][e] = n[e] > 0.f ? o[i][e] + add : o[i][e];
-                    }
-#pragma unroll
-                    for (int c = 0; c < 4; c++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-                        {
-                            unsigned x = a[c][e];
-                            x = (x & inf) == inf ? x & 0xffff0000u : x;
-                            x = (x >> 16 & inf) == inf ? x & 0xffffu : x;
-                            a[c][e] = x;
-                        }
-                }
+                if (__builtin_expect(__builtin_amdgcn_ballot_w64((bad & 0x80008000u) != 0) != 0, 0))
+                    o[i] = count_odd<NB>(a, k0, o[i]);
             }
 #pragma unroll
-            for (int c = 0; c < 4; c++)
+            for (int c = 0; c < 2 * NB; c++)
                 o[i] = IO::mfma(a[c], w[c], o[i]);
         }
     }
+    // Takes the values that are +Inf, -Inf or NaN out of a tile's operand and
+    // adds them to the sums of the rows that see one, by counting.
+    template <int NB>
+    __device__ f16v count_odd(u4 (&a)[2 * NB], int k0, f16v sum) const
+    {
+        constexpr unsigned kInf = IO::kExpMask & 0xffffu;
+#pragma nounroll
+        for (int kind = 0; kind < 3; kind++)
+        {
+            const unsigned want = kind == 0 ? kInf : kInf | 0x8000u;
+            auto flag = [&](unsigned x) {
+                const unsigned hit = kind < 2 ? x == want : (x & 0x7fffu) > kInf;
+                return hit ? IO::kOne : 0u;
+            };
+            f16v n;
+#pragma unroll
+            for (int e = 0; e < 16; e++)
+                n[e] = 0.f;
+#pragma unroll
+            for (int c = 0; c < 2 * NB; c++)
+            {
+                int first = key_of(k0, c >> 1, 8 * (c & 1));
+                asm volatile("" : "+v"(first)); // formed anew: kept, visibility outgrows the scalar registers
+                u4 is, vis;
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                {
+                    const int j = first + 8 * (e >> 1) + 2 * (e & 1);
+                    is[e] = flag(a[c][e] & 0xffffu) | flag(a[c][e] >> 16) << 16;
+                    vis[e] = (sees(j) ? IO::kOne : 0u) | (sees(j + 1) ? IO::kOne << 16 : 0u);
+                }
+                n = IO::mfma(is, vis, n);
+            }
+            const float extra = kind == 0 ? -kNegInf : kind == 1 ? kNegInf : __builtin_nanf("");
+#pragma unroll
+            for (int e = 0; e < 16; e++)
+                sum[e] = n[e] > 0.f ? sum[e] + extra : sum[e];
+        }
+#pragma unroll
+        for (int c = 0; c < 2 * NB; c++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+            {
+                a[c][e] = (a[c][e] & kInf) == kInf ? a[c][e] & 0xffff0000u : a[c][e];
+                a[c][e] = (a[c][e] >> 16 & kInf) == kInf ? a[c][e] & 0xffffu : a[c][e];
+            }
+        return sum;
+    }
+};
 
-    l = partner_sum(l);
-    if (!live)
+// Whether rows at positions p0 .. p1 do not all see all of n keys from k0 on.
+__device__ inline bool is_masked(const SlideParams& p, int nk, int p0, int p1, int k0, int n)
+{
+    return !(k0 + n <= nk && k0 + n - 1 <= p0 + p.right && (k0 + n <= p.sinks || k0 >= p1 - p.left));
+}
+
+// What a workgroup works on: XCD x (workgroup id mod 8) takes a contiguous run
+// of blocks, so that tiles of one key head share an L2.
+struct Place
+{
+    int tile, split, kvh, b, nq, nk, rows, off;
+    bool none;
+    __device__ explicit Place(const SlideParams& p, int tile_rows)
+    {
+        const int id = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+        none = id >= p.blocks;
+        tile = id % p.row_tiles;
+        int rest = id / p.row_tiles;
+        split = rest % p.splits;
+        rest /= p.splits;
+        kvh = rest % p.kv_heads;
+        b = none ? 0 : rest / p.kv_heads;
+        nq = __builtin_amdgcn_readfirstlane(clamp_len(p.q_lens, b, p.q_len));
+        nk = __builtin_amdgcn_readfirstlane(clamp_len(p.kv_lens, b, p.kv_len));
+        rows = nq * p.group;
+        off = nk - nq;
+        none = none || tile * tile_rows >= rows;
+    }
+};
+
+// Tile form: 128 rows by four waves of 32, tiles of 64 keys in two LDS
+// buffers, the next one on its way while one is worked on; one barrier a tile.
+template <typename IO, int D>
+__global__ __launch_bounds__(64 * kWaves, 2) void slide_tile_kernel(SlideParams p)
+{
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    constexpr int kRowBytes = 2 * D;
+    constexpr int kChunks = kRowBytes / 16;
+    constexpr int kTileBytes = kKeys * kRowBytes;
+    constexpr int kBuf = 2 * kTileBytes;
+    constexpr int kBlocks = D / 32;
+    constexpr int kRowsPerDma = 64 / kChunks;
+    constexpr int kDma = kKeys / kRowsPerDma / kWaves; // of each of K and V per wave
+
+    const Place at(p, kRows);
+    if (at.none)
         return;
-    const long long at = (static_cast<long long>(b) * p.heads + head) * p.q_len + qi;
+    const int first = at.tile * kRows;
+    const int p0 = at.off + first / p.group;
+    const int p1 = at.off + (min(first + kRows, at.rows) - 1) / p.group;
+    const KeyTiles<kKeys> kt(p, at.nk, p0, p1);
+    const int share = (kt.count + p.splits - 1) / p.splits;
+    const int t0 = min(at.split * share, kt.count);
+    const int t1 = min(t0 + share, kt.count);
+
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int row = first + wave * 32 + (lane & 31);
+    Rows<IO, D> r;
+    r.init(p, at.b, at.kvh, min(row, at.rows - 1), at.off, at.nk, lane);
+
+    const char* kb = p.k + at.b * p.k_b + at.kvh * p.k_h;
+    const char* vb = p.v + at.b * p.v_b + at.kvh * p.v_h;
+    const unsigned lds0 = static_cast<unsigned>(reinterpret_cast<size_t>(smem));
+    const unsigned k_step = static_cast<unsigned>(p.k_t);
+    const unsigned v_step = static_cast<unsigned>(p.v_t);
+    auto fetch = [&](int k0, int buf) {
+        const int last = at.nk - 1 - k0; // rows past the end repeat the last one
+        const char* kp = kb + k0 * p.k_t;
+        const char* vp = vb + k0 * p.v_t;
+        const unsigned d = lds0 + buf * kBuf;
+#pragma unroll
+        for (int i = 0; i < kDma; i++)
+        {
+            const int r0 = (wave * kDma + i) * kRowsPerDma;
+            const unsigned r = r0 + lane / kChunks;
+            const unsigned c = lane % kChunks;
+            const unsigned rr = min(static_cast<int>(r), last);
+            dma16(kp, rr * k_step + ((c ^ key_swz<D>(r)) << 4), d + r0 * kRowBytes);
+            dma16(vp, rr * v_step + ((c ^ value_swz<D>(r)) << 4), d + kTileBytes + r0 * kRowBytes);
+        }
+    };
+    if (t0 < t1)
+        fetch(kt.key(t0), 0);
+    for (int t = t0; t < t1; t++)
+    {
+        const int buf = (t - t0) & 1;
+        wait_vm<0>();
+        bar(); // the tile is whole, and the other buffer's readers are done
+        if (t + 1 < t1)
+            fetch(kt.key(t + 1), buf ^ 1);
+        const int k0 = kt.key(t);
+        const char* st = smem + buf * kBuf;
+        const bool masked = is_masked(p, at.nk, p0, p1, k0, kKeys);
+        f16v s[2];
+        u4 w[4];
+        r.template scores<2>(s, st);
+        if (masked)
+            r.template mask<2>(s, k0);
+        r.template weights<2>(s, w);
+        r.template add<2>(w, st + kTileBytes, k0, masked);
+    }
+
+    const float l = partner_sum(r.l);
+    if (row >= at.rows)
+        return;
+    const long long to = (static_cast<long long>(at.b) * p.heads + r.head) * p.q_len + r.qi;
     if (p.splits > 1)
     {
-        const long long to = static_cast<long long>(split) * p.batch * p.heads * p.q_len + at;
-        float* dst = p.part + to * D + 4 * half;
+        const long long part = static_cast<long long>(at.split) * p.batch * p.heads * p.q_len + to;
+        float* dst = p.part + part * D + 4 * r.half;
 #pragma unroll
         for (int i = 0; i < kBlocks; i++)
 #pragma unroll
             for (int e = 0; e < 4; e++)
                 *reinterpret_cast<float4*>(dst + 32 * i + 8 * e) =
-                    make_float4(o[i][4 * e], o[i][4 * e + 1], o[i][4 * e + 2], o[i][4 * e + 3]);
-        if (half == 0)
-            p.part_ml[to] = make_float2(m, l);
+                    make_float4(r.o[i][4 * e], r.o[i][4 * e + 1], r.o[i][4 * e + 2], r.o[i][4 * e + 3]);
+        if (r.half == 0)
+            p.part_ml[part] = make_float2(r.m, l);
         return;
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    char* dst = p.out + b * p.o_b + qi * p.o_t + head * p.o_h + 8 * half;
+    char* dst = p.out + at.b * p.o_b + r.qi * p.o_t + r.head * p.o_h + 8 * r.half;
 #pragma unroll
     for (int i = 0; i < kBlocks; i++)
 #pragma unroll
         for (int e = 0; e < 4; e++)
             *reinterpret_cast<u2*>(dst + 64 * i + 16 * e) =
-                u2{IO::pack(o[i][4 * e] * inv, o[i][4 * e + 1] * inv), IO::pack(o[i][4 * e + 2] * inv, o[i][4 * e + 3] * inv)};
-    if (p.lse && half == 0)
-        p.lse[at] = l == 0.f ? kNegInf : m * kLn2 + logf(l);
+                u2{IO::pack(r.o[i][4 * e] * inv, r.o[i][4 * e + 1] * inv), IO::pack(r.o[i][4 * e + 2] * inv, r.o[i][4 * e + 3] * inv)};
+    if (p.lse && r.half == 0)
+        p.lse[to] = l == 0.f ? kNegInf : r.m * kLn2 + logf(l);
 }
 
-// Joins the splits of one query row: one wave per row.
-template <typename IO, int D>
-__global__ __launch_bounds__(256) void slide_join_kernel(SlideParams p)
+// Few form, for at most 32 rows of a key head (single tokens): a stream of the
+// cache.  The four waves of a workgroup take tiles of 32 keys in turn, each
+// through LDS slots of its own with the next tiles on their way, so no barrier
+// stands in the stream; their sums are joined in LDS at the end.
+constexpr int kFewWaves = 2;
+template <int D>
+struct FewShape
 {
+    static constexpr int kTileBytes = 32 * 2 * D;
+    static constexpr int kSlots = D == 128 ? 2 : 4;
+    static constexpr int kWaveBytes = kSlots * 2 * kTileBytes; // 32 KB
+    static constexpr int kLds = kFewWaves * kWaveBytes;
+    static_assert(32 * (D + 4) * 4 + 256 <= kWaveBytes, "a wave's sums fit its slots");
+};
+
+template <typename IO, int D>
+__global__ __launch_bounds__(64 * kFewWaves) void slide_few_kernel(SlideParams p)
+{
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    using S = FewShape<D>;
+    constexpr int kRowBytes = 2 * D;
+    constexpr int kChunks = kRowBytes / 16;
+    constexpr int kBlocks = D / 32;
+    constexpr int kRowsPerDma = 64 / kChunks;
+    constexpr int kDma = 32 / kRowsPerDma; // of each of K and V per tile
+
+    const Place at(p, 32);
+    if (at.none)
+        return;
+    const int p0 = at.off;
+    const int p1 = at.off + at.nq - 1;
+    const KeyTiles<32> kt(p, at.nk, p0, p1);
+    const int share = (kt.count + p.splits - 1) / p.splits;
+    const int t0 = min(at.split * share, kt.count);
+    const int nt = min(share, kt.count - t0);
+
     const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int mine = wave < nt ? (nt - 1 - wave) / kFewWaves + 1 : 0; // tiles wave, wave + kFewWaves, ...
+
+    const char* kb = p.k + at.b * p.k_b + at.kvh * p.k_h;
+    const char* vb = p.v + at.b * p.v_b + at.kvh * p.v_h;
+    char* const ring = smem + wave * S::kWaveBytes;
+    const unsigned lds = static_cast<unsigned>(reinterpret_cast<size_t>(ring));
+    const unsigned k_step = static_cast<unsigned>(p.k_t);
+    const unsigned v_step = static_cast<unsigned>(p.v_t);
+    auto fetch = [&](int i) {
+        const int k0 = kt.key(t0 + wave + i * kFewWaves);
+        const int last = at.nk - 1 - k0; // rows past the end repeat the last one
+        const char* kp = kb + k0 * p.k_t;
+        const char* vp = vb + k0 * p.v_t;
+        const unsigned d = lds + (i % S::kSlots) * 2 * S::kTileBytes;
+#pragma unroll
+        for (int j = 0; j < kDma; j++)
+        {
+            const unsigned r = j * kRowsPerDma + lane / kChunks;
+            const unsigned c = lane % kChunks;
+            const unsigned rr = min(static_cast<int>(r), last);
+            dma16(kp, rr * k_step + ((c ^ key_swz<D>(r)) << 4), d + j * 1024);
+            dma16(vp, rr * v_step + ((c ^ value_swz<D>(r)) << 4), d + S::kTileBytes + j * 1024);
+        }
+    };
+    for (int i = 0; i < min(mine, S::kSlots - 1); i++)
+        fetch(i);
+    const int row = min(lane & 31, at.rows - 1);
+    Rows<IO, D> r;
+    r.init(p, at.b, at.kvh, row, at.off, at.nk, lane);
+    for (int i = 0; i < mine; i++)
+    {
+        if (i + S::kSlots - 1 < mine)
+        {
+            // the slot worked on before is free once its reads are done
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            fetch(i + S::kSlots - 1);
+            wait_vm<(S::kSlots - 1) * 2 * kDma>();
+        }
+        else
+            wait_vm<0>();
+        const int k0 = kt.key(t0 + wave + i * kFewWaves);
+        const char* st = ring + (i % S::kSlots) * 2 * S::kTileBytes;
+        const bool masked = is_masked(p, at.nk, p0, p1, k0, 32);
+        f16v s[1];
+        u4 w[2];
+        r.template scores<1>(s, st);
+        if (masked)
+            r.template mask<1>(s, k0);
+        r.template weights<1>(s, w);
+        r.template add<1>(w, st + S::kTileBytes, k0, masked);
+    }
+
+    // the waves' sums, relative to the largest maximum of a row
+    constexpr int kPitch = D + 4; // floats: rows start in different banks
+    float2* ml = reinterpret_cast<float2*>(ring + 32 * kPitch * 4);
+    float* sums = reinterpret_cast<float*>(ring);
+    const float l = partner_sum(r.l);
+    if ((lane & 31) < at.rows)
+    {
+#pragma unroll
+        for (int i = 0; i < kBlocks; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                *reinterpret_cast<float4*>(sums + (lane & 31) * kPitch + 32 * i + 8 * e + 4 * r.half) =
+                    make_float4(r.o[i][4 * e], r.o[i][4 * e + 1], r.o[i][4 * e + 2], r.o[i][4 * e + 3]);
+        if (r.half == 0)
+            ml[lane & 31] = make_float2(r.m, l);
+    }
+    __syncthreads();
+    for (int x = threadIdx.x; x < at.rows * (D / 4); x += 64 * kFewWaves)
+    {
+        const int rr = x / (D / 4);
+        const int d = 4 * (x % (D / 4));
+        float2 part[kFewWaves];
+        float m = kNegInf;
+#pragma unroll
+        for (int w = 0; w < kFewWaves; w++)
+        {
+            part[w] = reinterpret_cast<const float2*>(smem + w * S::kWaveBytes + 32 * kPitch * 4)[rr];
+            m = fmaxf(m, part[w].x);
+        }
+        const float base = m == kNegInf ? 0.f : m;
+        float total = 0.f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kFewWaves; w++)
+            if (part[w].y != 0.f) // else it saw no key
+            {
+                const float a = __builtin_amdgcn_exp2f(part[w].x - base);
+                const float4 u = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem + w * S::kWaveBytes) + rr * kPitch + d);
+                total += a * part[w].y;
+                v.x += a * u.x;
+                v.y += a * u.y;
+                v.z += a * u.z;
+                v.w += a * u.w;
+            }
+        const int qi = rr / p.group;
+        const int head = at.kvh * p.group + (rr - qi * p.group);
+        const long long to = (static_cast<long long>(at.b) * p.heads + head) * p.q_len + qi;
+        if (p.splits > 1)
+        {
+            const long long to_part = static_cast<long long>(at.split) * p.batch * p.heads * p.q_len + to;
+            *reinterpret_cast<float4*>(p.part + to_part * D + d) = v;
+            if (d == 0)
+                p.part_ml[to_part] = make_float2(m, total);
+            continue;
+        }
+        const float inv = total == 0.f ? 0.f : 1.f / total;
+        *reinterpret_cast<u2*>(p.out + at.b * p.o_b + qi * p.o_t + head * p.o_h + 2 * d) =
+            u2{IO::pack(v.x * inv, v.y * inv), IO::pack(v.z * inv, v.w * inv)};
+        if (p.lse && d == 0)
+            p.lse[to] = total == 0.f ? kNegInf : m * kLn2 + logf(total);
+    }
+}
+
+// Joins the splits of query rows: teams of 32 lanes (D / 32 dims each), `per`
+// teams to a row, each with a share of its splits; all of a team's loads are
+// under way before the first is used.
+constexpr int kTeams = 8;
+template <typename IO, int D>
+__global__ __launch_bounds__(32 * kTeams) void slide_join_kernel(SlideParams p, int per)
+{
+    constexpr int kE = D / 32;
+    typedef __attribute__((ext_vector_type(kE))) float fe;
+    __shared__ float2 s_ml[kTeams];
+    __shared__ fe s_sum[kTeams][32];
+    const int lane = threadIdx.x & 31;
+    const int team = threadIdx.x >> 5;
     const long long rows = static_cast<long long>(p.batch) * p.heads * p.q_len;
-    const long long at = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    if (at >= rows)
+    const long long at = static_cast<long long>(blockIdx.x) * (kTeams / per) + team / per;
+    const long long atc = at < rows ? at : rows - 1;
+    const int mine = team % per;
+    float m = kNegInf;
+    float l = 0.f;
+    fe o = {};
+    for (int s0 = mine; s0 < p.splits; s0 += 4 * per)
+    {
+        float2 ml[4];
+        fe v[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+        {
+            const int s = min(s0 + i * per, p.splits - 1);
+            ml[i] = p.part_ml[s * rows + atc];
+            v[i] = *reinterpret_cast<const fe*>(p.part + (s * rows + atc) * D + kE * lane);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (s0 + i * per < p.splits && ml[i].y != 0.f) // else it saw no key
+            {
+                const float next = fmaxf(m, ml[i].x);
+                const float base = next == kNegInf ? 0.f : next;
+                const float a = __builtin_amdgcn_exp2f(m - base);
+                const float c = __builtin_amdgcn_exp2f(ml[i].x - base);
+                m = next;
+                l = l * a + c * ml[i].y;
+                o = o * a + c * v[i];
+            }
+    }
+    s_sum[team][lane] = o;
+    if (lane == 0)
+        s_ml[team] = make_float2(m, l);
+    __syncthreads();
+    if (mine != 0 || at >= rows)
         return;
     const int qi = static_cast<int>(at % p.q_len);
     const long long bh = at / p.q_len;
@@ -515,47 +766,46 @@ __global__ __launch_bounds__(256) void slide_join_kernel(SlideParams p)
     const int b = static_cast<int>(bh / p.heads);
     if (qi >= clamp_len(p.q_lens, b, p.q_len))
         return;
-    float m = kNegInf;
-    for (int s = 0; s < p.splits; s++)
-        m = fmaxf(m, p.part_ml[s * rows + at].x);
-    const float base = m == kNegInf ? 0.f : m;
-    float l = 0.f;
-    constexpr int kPer = D / 64;
-    float o[kPer];
-#pragma unroll
-    for (int e = 0; e < kPer; e++)
-        o[e] = 0.f;
-    for (int s = 0; s < p.splits; s++)
+    for (int t = 1; t < per; t++)
     {
-        const float2 ml = p.part_ml[s * rows + at];
+        const float2 ml = s_ml[team + t];
         if (ml.y == 0.f)
-            continue; // no visible key in this split
-        const float a = __builtin_amdgcn_exp2f(ml.x - base);
-        l += a * ml.y;
-        const float* src = p.part + (s * rows + at) * D + kPer * lane;
-#pragma unroll
-        for (int e = 0; e < kPer; e++)
-            o[e] += a * src[e];
+            continue;
+        const float next = fmaxf(m, ml.x);
+        const float base = next == kNegInf ? 0.f : next;
+        const float a = __builtin_amdgcn_exp2f(m - base);
+        const float c = __builtin_amdgcn_exp2f(ml.x - base);
+        m = next;
+        l = l * a + c * ml.y;
+        o = o * a + c * s_sum[team + t][lane];
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    char* dst = p.out + b * p.o_b + qi * p.o_t + head * p.o_h + 2 * kPer * lane;
-    if constexpr (kPer == 2)
-        *reinterpret_cast<unsigned*>(dst) = IO::pack(o[0] * inv, o[1] * inv);
+    char* dst = p.out + b * p.o_b + qi * p.o_t + head * p.o_h + 2 * kE * lane;
+    if constexpr (kE == 4)
+        *reinterpret_cast<u2*>(dst) = u2{IO::pack(o[0] * inv, o[1] * inv), IO::pack(o[2] * inv, o[3] * inv)};
     else
-        *reinterpret_cast<uint16_t*>(dst) = static_cast<uint16_t>(IO::pack(o[0] * inv, 0.f));
+        *reinterpret_cast<unsigned*>(dst) = IO::pack(o[0] * inv, o[1] * inv);
     if (p.lse && lane == 0)
         p.lse[at] = l == 0.f ? kNegInf : m * kLn2 + logf(l);
 }
 
-// Splits of the keys where the row tiles alone leave CUs without work: two
-// workgroups a CU at most, two tiles of keys each at least.
-int plan_splits(const SlideParams& p, long long tiles)
+// The form, and splits of the keys where the rows alone leave CUs without
+// work: two workgroups a CU at most in the tile form (two fit), three in the
+// few form (one fits at a time, and sequences of unlike lengths even out), two
+// tiles of keys each at least.
+void plan_tiles(SlideParams* p)
 {
-    const long long positions = std::min<long long>(p.q_len, (kRows + p.group - 1) / p.group + 1);
-    const long long span = std::min<long long>(p.kv_len, static_cast<long long>(p.sinks) + p.left + p.right + positions + kKeys);
-    const long long keys = (span + kKeys - 1) / kKeys;
-    const long long want = 512 / std::max(1LL, tiles);
-    return static_cast<int>(std::max(1LL, std::min(want, keys / 2)));
+    const long long rows = static_cast<long long>(p->q_len) * p->group;
+    const long long heads = static_cast<long long>(p->kv_heads) * p->batch;
+    p->few = rows <= 32;
+    const int tile_rows = p->few ? 32 : kRows;
+    const int tile_keys = p->few ? 32 * kFewWaves : kKeys;
+    p->row_tiles = static_cast<int>((rows + tile_rows - 1) / tile_rows);
+    const long long positions = std::min<long long>(p->q_len, (tile_rows + p->group - 1) / p->group + 1);
+    const long long span = std::min<long long>(p->kv_len, static_cast<long long>(p->sinks) + p->left + p->right + positions + kKeys);
+    const long long keys = (span + tile_keys - 1) / tile_keys;
+    const long long want = (p->few ? 512 : 256) / std::max(1LL, p->row_tiles * heads);
+    p->splits = static_cast<int>(std::max(1LL, std::min(want, p->few ? keys : keys / 2)));
 }
 
 long long part_rows(const SlideParams& p)
@@ -593,10 +843,8 @@ int make_params(const sv2_sliding_attn_args* a, const char* what, SlideParams* o
     p.right = std::min(a->right, kMost - 1);
     p.sinks = std::min(a->sinks, kMost);
     p.scale2 = a->scale * kLog2e;
-    const long long rows = static_cast<long long>(p.q_len) * p.group;
-    p.row_tiles = static_cast<int>((rows + kRows - 1) / kRows);
+    plan_tiles(&p);
     const long long tiles = static_cast<long long>(p.row_tiles) * p.kv_heads * p.batch;
-    p.splits = plan_splits(p, tiles);
     if (tiles * p.splits > INT_MAX - 8)
         return set_error(SV2_EUNSUPPORTED, std::string(what) + ": too many tiles");
     p.blocks = static_cast<int>(tiles * p.splits);
@@ -612,16 +860,21 @@ long long workspace_of(const SlideParams& p, int head_dim)
 template <typename IO, int D>
 int run_slide(const SlideParams& p, hipStream_t stream)
 {
-    constexpr int kLds = 2 * 2 * kKeys * 2 * D;
-    const int rc = set_dynamic_lds(reinterpret_cast<const void*>(&slide_tile_kernel<IO, D>), kLds, "slide_tile: dynamic LDS attribute");
+    const int lds = p.few ? FewShape<D>::kLds : 2 * 2 * kKeys * 2 * D;
+    auto kernel = p.few ? &slide_few_kernel<IO, D> : &slide_tile_kernel<IO, D>;
+    const int rc = set_dynamic_lds(reinterpret_cast<const void*>(kernel), lds, "sv2_sliding_attention: dynamic LDS attribute");
     if (rc != SV2_OK)
         return rc;
     const unsigned grid = (static_cast<unsigned>(p.blocks) + 7) / 8 * 8;
-    hipLaunchKernelGGL((slide_tile_kernel<IO, D>), dim3(grid), dim3(64 * kWaves), kLds, stream, p);
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(64 * (p.few ? kFewWaves : kWaves)), lds, stream, p);
     if (p.splits > 1)
     {
         const long long rows = static_cast<long long>(p.batch) * p.heads * p.q_len;
-        hipLaunchKernelGGL((slide_join_kernel<IO, D>), dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), 0, stream, p);
+        const int per = p.splits > 8 ? 8 : p.splits > 4 ? 2 : 1;
+        const long long grid = (rows + kTeams / per - 1) / (kTeams / per);
+        if (grid > INT_MAX)
+            return set_error(SV2_EUNSUPPORTED, "sv2_sliding_attention: too many rows");
+        hipLaunchKernelGGL((slide_join_kernel<IO, D>), dim3(static_cast<unsigned>(grid)), dim3(32 * kTeams), 0, stream, p, per);
     }
     const hipError_t err = hipGetLastError();
     return err == hipSuccess ? SV2_OK : hip_error(err, "sv2_sliding_attention launch");
@@ -658,15 +911,23 @@ try
     if (misaligned(a.q, 16) || misaligned(a.k, 16) || misaligned(a.v, 16) || misaligned(a.out, 16) ||
         misaligned(a.q_lens, 4) || misaligned(a.kv_lens, 4) || misaligned(a.lse, 4))
         return set_error(SV2_EINVAL, "sv2_sliding_attention: q, k, v and out must be 16-byte aligned, the rest 4-byte");
-    const int64_t strides[12] = {a.q_batch_stride, a.q_token_stride, a.q_head_stride, a.k_batch_stride, a.k_token_stride,
-                                 a.k_head_stride, a.v_batch_stride, a.v_token_stride, a.v_head_stride,
-                                 a.out_batch_stride, a.out_token_stride, a.out_head_stride};
-    for (int64_t s : strides)
+    // of a dimension of one element the stride says nothing
+    const int64_t extents[12] = {a.batch, a.q_len, a.heads, a.batch, a.kv_len, a.kv_heads, a.batch, a.kv_len, a.kv_heads,
+                                 a.batch, a.q_len, a.heads};
+    int64_t strides[12] = {a.q_batch_stride, a.q_token_stride, a.q_head_stride, a.k_batch_stride, a.k_token_stride,
+                           a.k_head_stride, a.v_batch_stride, a.v_token_stride, a.v_head_stride,
+                           a.out_batch_stride, a.out_token_stride, a.out_head_stride};
+    for (int i = 0; i < 12; i++)
+    {
+        if (extents[i] <= 1)
+            strides[i] = 0;
+        const int64_t s = strides[i];
         if (s < 0 || s % 8 != 0 || s > INT64_MAX / 4)
             return set_error(SV2_EINVAL, "sv2_sliding_attention: strides must be non-negative multiples of 8 elements");
+    }
     // a tile's rows are addressed by 32-bit offsets from its first
     constexpr int64_t kMostStride = INT32_MAX / (2 * kKeys) - 256;
-    if (a.k_token_stride > kMostStride || a.v_token_stride > kMostStride)
+    if (strides[4] > kMostStride || strides[7] > kMostStride)
         return set_error(SV2_EUNSUPPORTED, "sv2_sliding_attention: token stride of k or v above 2^24 elements");
     const long long need = workspace_of(p, a.head_dim);
     if (need > 0 && (!a.workspace || a.workspace_bytes < static_cast<size_t>(need) || misaligned(a.workspace, 16)))

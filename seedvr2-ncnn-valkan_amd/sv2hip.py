@@ -1160,25 +1160,21 @@ def inner_product_f16_few(x, w, y, epilogue=EPI_STORE, w_value=None, bias=None, 
 
 
 def _need(name, t, dtype, shape, device):
-    """A tensor of this type, shape and device whose last dimension is
-    contiguous."""
-    if t.dtype != dtype or t.shape != shape or t.device != device or (shape[-1] > 1 and t.stride(-1) != 1):
+    """The address and the strides of a tensor of this type, shape and device
+    whose last dimension is contiguous."""
+    step = t.stride()
+    if t.dtype is not dtype or t.shape != shape or (step[-1] != 1 and shape[-1] > 1) or t.device != device:
         raise ValueError(f"{name} must be a {dtype} tensor {tuple(shape)} on {device} with a contiguous last dimension")
+    return t.data_ptr(), *step[:-1]
 
 
 def _dense_ptr(name, t, dtype, shape, device):
     """The address of an optional contiguous tensor."""
     if t is None:
         return None
-    if t.dtype != dtype or t.shape != shape or t.device != device or not t.is_contiguous():
+    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous() or t.device != device:
         raise ValueError(f"{name} must be a contiguous {dtype} tensor {tuple(shape)} on {device}")
     return t.data_ptr()
-
-
-def _steps(t):
-    """Strides of all but the last dimension; 0 where there is nothing to step
-    over."""
-    return [s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape[:-1])]
 
 
 def _row_step(t):
@@ -1242,16 +1238,13 @@ def sliding_attention(q, k, v, out, *, left, right=0, sinks=0, scale=None, q_len
     b, nq, h, d = shape
     _, nk, g, _ = k.shape
     dtype, dev = q.dtype, q.device
-    _need("q", q, dtype, shape, dev)
-    _need("k", k, dtype, (b, nk, g, d), dev)
-    _need("v", v, dtype, (b, nk, g, d), dev)
-    _need("out", out, dtype, shape, dev)
+    cache = (b, nk, g, d)
     most = 2**31 - 1
     a = SlidingAttnArgs(b, nq, nk, h, g, d, _code(q), min(left, most), min(right, most), min(sinks, most),
                         d ** -0.5 if scale is None else scale,
-                        q.data_ptr(), *_steps(q), k.data_ptr(), *_steps(k), v.data_ptr(), *_steps(v),
-                        out.data_ptr(), *_steps(out), _dense_ptr("q_lens", q_lens, torch.int32, (b,), dev),
-                        _dense_ptr("kv_lens", kv_lens, torch.int32, (b,), dev),
+                        *_need("q", q, dtype, shape, dev), *_need("k", k, dtype, cache, dev),
+                        *_need("v", v, dtype, cache, dev), *_need("out", out, dtype, shape, dev),
+                        _dense_ptr("q_lens", q_lens, torch.int32, (b,), dev), _dense_ptr("kv_lens", kv_lens, torch.int32, (b,), dev),
                         _dense_ptr("lse", lse, torch.float32, (b, h, nq), dev))
     lib = load()
     ref = ctypes.byref(a)
