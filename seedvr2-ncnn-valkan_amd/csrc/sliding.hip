@@ -208,6 +208,10 @@ __device__ inline unsigned value_swz(unsigned r)
     return D == 128 ? (r & 3) << 2 : ((r >> 1) & 1) << 2;
 }
 
+// Largest rise of a row's maximum, in powers of two, that its weights absorb:
+// up to 2^8, far inside both types.
+constexpr float kRise = 8.f;
+
 // 32 query rows in one wave: lane % 32 is the row (its two half-waves hold
 // different keys of the scores and different dims of the sums).
 template <typename IO, int D>
@@ -219,7 +223,7 @@ struct Rows
 
     u4 q[kSteps];
     f16v o[kBlocks]; // sums, dims 32 i + 8 (e / 4) + 4 half + e % 4
-    float m;         // largest score so far, times scale2
+    float m;         // the largest score in use, times scale2
     float l;         // this half-wave's part of the sum of weights
     int half, qi, head, hi_key, lo_key, sinks;
     float scale2;
@@ -270,13 +274,28 @@ struct Rows
     {
 #pragma unroll
         for (int i = 0; i < NB; i++)
-        {
 #pragma unroll
             for (int e = 0; e < 16; e++)
                 s[i][e] = 0.f;
+        // the blocks in turn (a product that waits for the one before it costs
+        // the matrix unit its latency), operands read kAhead products ahead: the
+        // compiler, left to itself, reads each where it is used
+        constexpr int kAhead = 3;
+        constexpr int kAll = NB * kSteps;
+        u4 a[kAhead + 1];
+        auto read = [&](int j) {
+            a[j % (kAhead + 1)] = *reinterpret_cast<const u4*>(keys + (j % NB) * 32 * kRowBytes + koff[j / NB]);
+        };
 #pragma unroll
-            for (int c = 0; c < kSteps; c++)
-                s[i] = IO::mfma(*reinterpret_cast<const u4*>(keys + i * 32 * kRowBytes + koff[c]), q[c], s[i]);
+        for (int j = 0; j < kAhead; j++)
+            read(j);
+#pragma unroll
+        for (int j = 0; j < kAll; j++)
+        {
+            if (j + kAhead < kAll)
+                read(j + kAhead);
+            s[j % NB] = IO::mfma(a[j % (kAhead + 1)], q[j / NB], s[j % NB]);
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
     template <int NB>
@@ -300,8 +319,11 @@ struct Rows
             for (int e = 0; e < 16; e++)
                 s[i][e] = sees(key_of(k0, i, e)) ? s[i][e] : kNegInf;
     }
-    // scores to weights exp2(s scale2 - m), rounded for the product; the sums
-    // so far are rescaled when some row's maximum rose
+    // scores to weights exp2(s scale2 - m), rounded for the product.  m is the
+    // largest score but for a rise of up to kRise that the weights absorb; the
+    // sums are rescaled when some row's maximum rises further (of 32 rows one
+    // finds a larger score in nearly every tile: rescaling for each costs a
+    // quarter of the vector work)
     template <int NB>
     __device__ void weights(f16v (&s)[NB], u4 (&w)[2 * NB])
     {
@@ -312,7 +334,7 @@ struct Rows
             for (int e = 0; e < 16; e++)
                 top = fmaxf(top, s[i][e]);
         top = partner_max(top) * scale2;
-        if (__builtin_amdgcn_ballot_w64(top > m) != 0)
+        if (__builtin_amdgcn_ballot_w64(top - m > kRise) != 0)
         {
             const float next = fmaxf(top, m);
             const float alpha = next == kNegInf ? 1.f : __builtin_amdgcn_exp2f(m - next);
@@ -346,40 +368,52 @@ struct Rows
         const u2 hi = keys4(vals + voff[i] + (16 * c + 8) * kRowBytes);
         return u4{lo.x, lo.y, hi.x, hi.y};
     }
-    // sums += weights values; in a masked tile (from key k0 on) values that
-    // are not finite stay out of the product
-    template <int NB>
-    __device__ void add(const u4 (&w)[2 * NB], const char* vals, int k0, bool masked)
+    // the operands of 16 keys from 16 c on
+    __device__ void read_values(u4 (&a)[kBlocks], const char* vals, int c) const
     {
 #pragma unroll
         for (int i = 0; i < kBlocks; i++)
-        {
-            u4 a[2 * NB];
+            a[i] = values(vals, i, c);
+    }
+    // sums += weights values (`first`: the operands of the first 16 keys); in
+    // a masked tile (from key k0 on) values that are not finite stay out of
+    // the product
+    template <int NB>
+    __device__ void add(const u4 (&w)[2 * NB], u4 (&first)[kBlocks], const char* vals, int k0, bool masked)
+    {
+        u4 next[kBlocks];
 #pragma unroll
-            for (int c = 0; c < 2 * NB; c++)
-                a[c] = values(vals, i, c);
+        for (int c = 0; c < 2 * NB; c++)
+        {
+            u4(&a)[kBlocks] = c & 1 ? next : first;
+            if (c + 1 < 2 * NB)
+                read_values(c & 1 ? first : next, vals, c + 1);
+            __builtin_amdgcn_sched_barrier(0);
             if (masked)
             {
                 unsigned bad = 0;
 #pragma unroll
-                for (int c = 0; c < 2 * NB; c++)
+                for (int i = 0; i < kBlocks; i++)
 #pragma unroll
                     for (int e = 0; e < 4; e++)
-                        bad |= (a[c][e] & IO::kExpMask) + IO::kExpOne;
+                        bad |= (a[i][e] & IO::kExpMask) + IO::kExpOne;
                 if (__builtin_expect(__builtin_amdgcn_ballot_w64((bad & 0x80008000u) != 0) != 0, 0))
-                    o[i] = count_odd<NB>(a, k0, o[i]);
+#pragma unroll
+                    for (int i = 0; i < kBlocks; i++)
+                        count_odd(a[i], key_of(k0, c >> 1, 8 * (c & 1)), o[i]);
             }
 #pragma unroll
-            for (int c = 0; c < 2 * NB; c++)
-                o[i] = IO::mfma(a[c], w[c], o[i]);
+            for (int i = 0; i < kBlocks; i++)
+                o[i] = IO::mfma(a[i], w[c], o[i]);
         }
     }
-    // Takes the values that are +Inf, -Inf or NaN out of a tile's operand and
-    // adds them to the sums of the rows that see one, by counting.
-    template <int NB>
-    __device__ f16v count_odd(u4 (&a)[2 * NB], int k0, f16v sum) const
+    // Takes the values that are +Inf, -Inf or NaN out of an operand (of 16
+    // keys, this lane's from `first` on) and adds them to the sums of the rows
+    // that see one, by counting.
+    __device__ void count_odd(u4& a, int first, f16v& sum) const
     {
         constexpr unsigned kInf = IO::kExpMask & 0xffffu;
+        asm volatile("" : "+v"(first)); // formed anew: kept, visibility outgrows the scalar registers
 #pragma nounroll
         for (int kind = 0; kind < 3; kind++)
         {
@@ -388,39 +422,30 @@ struct Rows
                 const unsigned hit = kind < 2 ? x == want : (x & 0x7fffu) > kInf;
                 return hit ? IO::kOne : 0u;
             };
+            u4 is, vis;
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+            {
+                const int j = first + 8 * (e >> 1) + 2 * (e & 1);
+                is[e] = flag(a[e] & 0xffffu) | flag(a[e] >> 16) << 16;
+                vis[e] = (sees(j) ? IO::kOne : 0u) | (sees(j + 1) ? IO::kOne << 16 : 0u);
+            }
             f16v n;
 #pragma unroll
             for (int e = 0; e < 16; e++)
                 n[e] = 0.f;
-#pragma unroll
-            for (int c = 0; c < 2 * NB; c++)
-            {
-                int first = key_of(k0, c >> 1, 8 * (c & 1));
-                asm volatile("" : "+v"(first)); // formed anew: kept, visibility outgrows the scalar registers
-                u4 is, vis;
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                {
-                    const int j = first + 8 * (e >> 1) + 2 * (e & 1);
-                    is[e] = flag(a[c][e] & 0xffffu) | flag(a[c][e] >> 16) << 16;
-                    vis[e] = (sees(j) ? IO::kOne : 0u) | (sees(j + 1) ? IO::kOne << 16 : 0u);
-                }
-                n = IO::mfma(is, vis, n);
-            }
+            n = IO::mfma(is, vis, n);
             const float extra = kind == 0 ? -kNegInf : kind == 1 ? kNegInf : __builtin_nanf("");
 #pragma unroll
             for (int e = 0; e < 16; e++)
                 sum[e] = n[e] > 0.f ? sum[e] + extra : sum[e];
         }
 #pragma unroll
-        for (int c = 0; c < 2 * NB; c++)
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-            {
-                a[c][e] = (a[c][e] & kInf) == kInf ? a[c][e] & 0xffff0000u : a[c][e];
-                a[c][e] = (a[c][e] >> 16 & kInf) == kInf ? a[c][e] & 0xffffu : a[c][e];
-            }
-        return sum;
+        for (int e = 0; e < 4; e++)
+        {
+            a[e] = (a[e] & kInf) == kInf ? a[e] & 0xffff0000u : a[e];
+            a[e] = (a[e] >> 16 & kInf) == kInf ? a[e] & 0xffffu : a[e];
+        }
     }
 };
 
@@ -523,8 +548,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void slide_tile_kernel(SlideParams 
         r.template scores<2>(s, st);
         if (masked)
             r.template mask<2>(s, k0);
+        u4 v0[Rows<IO, D>::kBlocks];
+        r.read_values(v0, st + kTileBytes, 0);
         r.template weights<2>(s, w);
-        r.template add<2>(w, st + kTileBytes, k0, masked);
+        r.template add<2>(w, v0, st + kTileBytes, k0, masked);
     }
 
     const float l = partner_sum(r.l);
@@ -643,8 +670,10 @@ __global__ __launch_bounds__(64 * kFewWaves) void slide_few_kernel(SlideParams p
         r.template scores<1>(s, st);
         if (masked)
             r.template mask<1>(s, k0);
+        u4 v0[Rows<IO, D>::kBlocks];
+        r.read_values(v0, st + S::kTileBytes, 0);
         r.template weights<1>(s, w);
-        r.template add<1>(w, st + S::kTileBytes, k0, masked);
+        r.template add<1>(w, v0, st + S::kTileBytes, k0, masked);
     }
 
     // the waves' sums, relative to the largest maximum of a row
