@@ -14,7 +14,8 @@
 //         fetches whole 128-byte lines of w and x straight into a ring of LDS
 //         slots of its own, so no barrier stands in the stream; the four
 //         partial sums meet in LDS at the end.  One launch, no workspace.
-//   any   more rows: 128 x 128 tiles through registers.
+//   any   more rows whose operands the tile kernel of the inner products does
+//         not take: tiles through registers.
 #include "sv2_internal.h"
 #include "activation.h"
 #include "vec_io.h"
@@ -67,9 +68,7 @@ struct LinearParams
     int vec4; // rows of y and the residual hold whole aligned groups of 4
 };
 
-constexpr int kTile = 128;
-constexpr int kBK = 32;
-constexpr int kPitch = kBK * 2 + 16; // bytes of an LDS row: 16 rows of one chunk start in different banks
+constexpr int kBK = 64; // K of a step: whole 128-byte lines of every row
 
 // 8 elements of a row from column k on, zeros past `k_end`.
 __device__ inline u4 load8(const uint16_t* row, int k, int k_end)
@@ -90,40 +89,33 @@ __device__ inline void finish4(const LinearParams& p, int m, int n, f4 v, A act)
 {
     if (m >= p.m || n >= p.n)
         return;
+    const int left = p.n - n;
+    if (p.bias)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            v[e] += p.bias[min(n + e, p.n - 1)];
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        v[e] = act(v[e]);
     uint16_t* y = p.y + m * p.ldy + n;
     const uint16_t* r = p.r ? p.r + m * p.ldr + n : nullptr;
     if (p.vec4)
     {
-        u2 old = {0u, 0u};
         if (r)
-            old = *reinterpret_cast<const u2*>(r);
-        uint16_t o[4];
-#pragma unroll
-        for (int e = 0; e < 4; e++)
         {
-            float t = v[e];
-            if (p.bias)
-                t += p.bias[n + e];
-            t = act(t);
-            if (r)
-                t += IO::to_float(static_cast<uint16_t>(old[e >> 1] >> (16 * (e & 1))));
-            o[e] = IO::from_float(t);
+            const u2 old = *reinterpret_cast<const u2*>(r);
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                v[e] += IO::to_float(static_cast<uint16_t>(old[e >> 1] >> (16 * (e & 1))));
         }
-        *reinterpret_cast<u2*>(y) = u2{o[0] | static_cast<unsigned>(o[1]) << 16, o[2] | static_cast<unsigned>(o[3]) << 16};
+        *reinterpret_cast<u2*>(y) = u2{IO::from_float(v[0]) | static_cast<unsigned>(IO::from_float(v[1])) << 16,
+                                       IO::from_float(v[2]) | static_cast<unsigned>(IO::from_float(v[3])) << 16};
         return;
     }
 #pragma unroll
     for (int e = 0; e < 4; e++)
-        if (n + e < p.n)
-        {
-            float t = v[e];
-            if (p.bias)
-                t += p.bias[n + e];
-            t = act(t);
-            if (r)
-                t += IO::to_float(r[e]);
-            y[e] = IO::from_float(t);
-        }
+        if (e < left)
+            y[e] = IO::from_float(r ? v[e] + IO::to_float(r[e]) : v[e]);
 }
 
 // The activation by a uniform branch, for epilogues that are a small part of
@@ -306,102 +298,163 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_few_kernel(LinearParams
     }
 }
 
-// 128 x 128 outputs by 4 waves of 64 x 64, K in steps of 32 through registers
-// into two LDS buffers.
-template <typename IO, int ACT>
-__global__ __launch_bounds__(256, 2) void linear_any_kernel(LinearParams p)
+// Any form: TILE x TILE outputs by 4 waves, K in steps of 64 through registers
+// (three steps ahead of their use) into two LDS buffers.  16-byte loads at any
+// element alignment; only the last step looks at K's end.
+template <int TILE>
+struct AnyShape
 {
-    __shared__ __attribute__((aligned(16))) char smem[2][2][kTile * kPitch];
+    static constexpr int kPitch = kBK * 2 + 16; // bytes of an LDS row: 16 rows of one chunk start in different banks
+    static constexpr int kOperand = TILE * kPitch;
+    static constexpr int kLds = 2 * 2 * kOperand;
+    static constexpr int kPieces = TILE * 8 / 256; // 16-byte pieces of an operand per thread and step
+};
+
+template <typename IO, int ACT, int TILE>
+__global__ __launch_bounds__(256, TILE == 128 ? 2 : 4) void linear_any_kernel(LinearParams p)
+{
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    using S = AnyShape<TILE>;
+    constexpr int kPieces = S::kPieces;
+    constexpr int kPart = TILE / 2; // of a wave, each way
+    constexpr int kT = kPart / 16;
     const int tn = blockIdx.x % p.tiles_n;
     const int tm = blockIdx.x / p.tiles_n;
-    const int m0 = tm * kTile;
-    const int n0 = tn * kTile;
+    const int m0 = tm * TILE;
+    const int n0 = tn * TILE;
     const int lane = threadIdx.x & 63;
     const int wave = threadIdx.x >> 6;
     const int lr = lane & 15;
     const int lq = lane >> 4;
-    const int wn = 64 * (wave & 1);
-    const int wm = 64 * (wave >> 1);
+    const int wn = kPart * (wave & 1);
+    const int wm = kPart * (wave >> 1);
 
-    // this thread's chunks: rows threadIdx / 4 and + 64, chunk threadIdx % 4
-    const int cr = threadIdx.x >> 2;
-    const int cc = threadIdx.x & 3;
-    const uint16_t* xr[2];
-    const uint16_t* wr[2];
+    // this thread's pieces: rows threadIdx / 8 + 32 i, chunk threadIdx % 8
+    const int cr = threadIdx.x >> 3;
+    const int cc = threadIdx.x & 7;
+    const uint16_t* xr[kPieces];
+    const uint16_t* wr[kPieces];
 #pragma unroll
-    for (int i = 0; i < 2; i++)
+    for (int i = 0; i < kPieces; i++)
     {
         // rows past the end repeat the last one; their sums are not stored
-        xr[i] = p.x + min(m0 + cr + 64 * i, p.m - 1) * p.ldx;
-        wr[i] = p.w + min(n0 + cr + 64 * i, p.n - 1) * p.ldw;
+        xr[i] = p.x + min(m0 + cr + 32 * i, p.m - 1) * p.ldx;
+        wr[i] = p.w + min(n0 + cr + 32 * i, p.n - 1) * p.ldw;
     }
-    u4 xv[2], wv[2];
-    auto load = [&](int k0) {
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-        {
-            xv[i] = load8(xr[i], k0 + 8 * cc, p.k);
-            wv[i] = load8(wr[i], k0 + 8 * cc, p.k);
-        }
-    };
-    auto put = [&](int buf) {
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-        {
-            *reinterpret_cast<u4*>(&smem[buf][0][(cr + 64 * i) * kPitch + 16 * cc]) = wv[i];
-            *reinterpret_cast<u4*>(&smem[buf][1][(cr + 64 * i) * kPitch + 16 * cc]) = xv[i];
-        }
-    };
-    f4 acc[4][4];
-#pragma unroll
-    for (int t = 0; t < 4; t++)
-#pragma unroll
-        for (int b = 0; b < 4; b++)
-            acc[t][b] = f4{0.f, 0.f, 0.f, 0.f};
-    load(0);
-    put(0);
-    __syncthreads();
     const int steps = (p.k + kBK - 1) / kBK;
-    for (int s = 0; s < steps; s++)
+    struct Held
     {
-        const int buf = s & 1;
-        if (s + 1 < steps)
-            load((s + 1) * kBK);
-        u4 a[4], b[4];
-#pragma unroll
-        for (int t = 0; t < 4; t++)
+        u4 x[kPieces], w[kPieces];
+    };
+    auto load = [&](Held& h, int s) {
+        const int k = s * kBK + 8 * cc;
+        if ((s + 1) * kBK <= p.k)
         {
-            a[t] = *reinterpret_cast<const u4*>(&smem[buf][0][(wn + 16 * t + lr) * kPitch + 16 * lq]);
-            b[t] = *reinterpret_cast<const u4*>(&smem[buf][1][(wm + 16 * t + lr) * kPitch + 16 * lq]);
+#pragma unroll
+            for (int i = 0; i < kPieces; i++)
+            {
+                h.x[i] = *reinterpret_cast<const u4u*>(xr[i] + k);
+                h.w[i] = *reinterpret_cast<const u4u*>(wr[i] + k);
+            }
         }
+        else if (s < steps)
+        {
 #pragma unroll
-        for (int t = 0; t < 4; t++)
+            for (int i = 0; i < kPieces; i++)
+            {
+                h.x[i] = load8(xr[i], k, p.k);
+                h.w[i] = load8(wr[i], k, p.k);
+            }
+        }
+    };
+    auto put = [&](const Held& h, int s) {
+        char* to = smem + (s & 1) * 2 * S::kOperand + cr * S::kPitch + 16 * cc;
 #pragma unroll
-            for (int u = 0; u < 4; u++)
-                acc[t][u] = IO::mfma(a[t], b[u], acc[t][u]);
+        for (int i = 0; i < kPieces; i++)
+        {
+            *reinterpret_cast<u4*>(to + 32 * i * S::kPitch) = h.w[i];
+            *reinterpret_cast<u4*>(to + S::kOperand + 32 * i * S::kPitch) = h.x[i];
+        }
+    };
+    f4 acc[kT][kT];
+#pragma unroll
+    for (int t = 0; t < kT; t++)
+#pragma unroll
+        for (int u = 0; u < kT; u++)
+            acc[t][u] = f4{0.f, 0.f, 0.f, 0.f};
+    auto multiply = [&](int s) {
+        const char* from = smem + (s & 1) * 2 * S::kOperand + lr * S::kPitch + 16 * lq;
+#pragma unroll
+        for (int ks = 0; ks < 2; ks++)
+        {
+            u4 a[kT], b[kT];
+#pragma unroll
+            for (int t = 0; t < kT; t++)
+            {
+                a[t] = *reinterpret_cast<const u4*>(from + (wn + 16 * t) * S::kPitch + 64 * ks);
+                b[t] = *reinterpret_cast<const u4*>(from + S::kOperand + (wm + 16 * t) * S::kPitch + 64 * ks);
+            }
+#pragma unroll
+            for (int t = 0; t < kT; t++)
+#pragma unroll
+                for (int u = 0; u < kT; u++)
+                    acc[t][u] = IO::mfma(a[t], b[u], acc[t][u]);
+        }
+    };
+    // step s: the next one's registers go to LDS, and are loaded for step s + 3
+    auto step = [&](Held& h, int s) {
         if (s + 1 < steps)
-            put(buf ^ 1);
+            put(h, s + 1);
+        load(h, s + 3);
+        multiply(s);
         __syncthreads();
+    };
+    Held even, odd;
+    load(even, 0);
+    load(odd, 1);
+    put(even, 0);
+    load(even, 2);
+    __syncthreads();
+    for (int s = 0; s < steps; s += 2)
+    {
+        step(odd, s);
+        if (s + 1 < steps)
+            step(even, s + 1);
     }
 #pragma unroll
-    for (int t = 0; t < 4; t++)
+    for (int t = 0; t < kT; t++)
 #pragma unroll
-        for (int u = 0; u < 4; u++)
+        for (int u = 0; u < kT; u++)
             finish4<IO>(p, m0 + wm + 16 * u + lr, n0 + wn + 16 * t + 4 * lq, acc[t][u],
                         [](float v) { return activate<ACT, false>(v); });
 }
 
-template <typename IO, int ACT>
-int run_linear(LinearParams p, hipStream_t stream)
+template <typename IO, int ACT, int TILE>
+int run_any(LinearParams p, hipStream_t stream)
 {
-    p.tiles_m = (p.m + kTile - 1) / kTile;
-    p.tiles_n = (p.n + kTile - 1) / kTile;
+    p.tiles_m = (p.m + TILE - 1) / TILE;
+    p.tiles_n = (p.n + TILE - 1) / TILE;
     const long long total = static_cast<long long>(p.tiles_m) * p.tiles_n;
     if (total > INT_MAX)
         return set_error(SV2_EUNSUPPORTED, "sv2_linear: too many tiles");
-    hipLaunchKernelGGL((linear_any_kernel<IO, ACT>), dim3(static_cast<unsigned>(total)), dim3(256), 0, stream, p);
+    const int rc = set_dynamic_lds(reinterpret_cast<const void*>(&linear_any_kernel<IO, ACT, TILE>), AnyShape<TILE>::kLds,
+                                   "linear_any: dynamic LDS attribute");
+    if (rc != SV2_OK)
+        return rc;
+    hipLaunchKernelGGL((linear_any_kernel<IO, ACT, TILE>), dim3(static_cast<unsigned>(total)), dim3(256),
+                       AnyShape<TILE>::kLds, stream, p);
     const hipError_t err = hipGetLastError();
     return err == hipSuccess ? SV2_OK : hip_error(err, "sv2_linear launch");
+}
+
+template <typename IO, int ACT>
+int run_linear(const LinearParams& p, hipStream_t stream)
+{
+    // the large tile where it has three rounds of CUs and more: 16000 x 2561 ->
+    // 2561 (2625 tiles) takes 631 us in it and 677 in the small one, 4000 rows
+    // (672 tiles) 177 and 178, 2000 rows (336) 118 and 101
+    const long long tiles = ((p.m + 127LL) / 128) * ((p.n + 127LL) / 128);
+    return tiles >= 768 ? run_any<IO, ACT, 128>(p, stream) : run_any<IO, ACT, 64>(p, stream);
 }
 
 template <typename IO, int MT, int CT, bool WHOLE>
