@@ -1196,6 +1196,11 @@ bool linear_tiles_fit(const LinearOperands& o)
            o.ldw < kMostStride && !misaligned(o.x, 16) && !misaligned(o.w, 16) && !misaligned(o.y, 16) && !misaligned(o.r, 16);
 }
 
+double linear_tiles_us(const LinearOperands& o)
+{
+    return make_plan(o.m, o.k, o.n, kGemmLinear, false).us;
+}
+
 int linear_tiles(hipStream_t stream, const LinearOperands& o)
 {
     TileArgs a{};

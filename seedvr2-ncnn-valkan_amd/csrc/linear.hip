@@ -8,7 +8,8 @@
 // columns of one output row.
 //
 // Two forms, by the number of rows.
-//   few   up to 64 rows: a stream of w.  A workgroup of four waves takes 16 CT
+//   few   up to 64 rows, and some blocks of 64 where these leave tiles few: a
+//         stream of w.  A workgroup of four waves takes 16 CT
 //         columns and splits K among its waves in blocks of 64 (interleaved:
 //         together they read 512 consecutive bytes of a row).  Each wave
 //         fetches whole 128-byte lines of w and x straight into a ring of LDS
@@ -22,6 +23,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <cmath>
 
 namespace sv2
 {
@@ -156,6 +158,7 @@ __device__ inline void wait_vm()
 
 constexpr int kFewWaves = 4;
 constexpr int kFewRows = 64;
+constexpr int kFewMost = 1024; // rows the few form is weighed for
 
 // The few form's LDS: a ring of slots of 16 CT rows of w and 16 MT rows of x,
 // 128 bytes each, per wave; 16-byte chunk c of row r sits in slot c ^ (r & 7),
@@ -185,6 +188,12 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_few_kernel(LinearParams
     const int lr = lane & 15;
     const int lq = lane >> 4;
     const int n0 = blockIdx.x * 16 * CT;
+    const int m0 = blockIdx.y * kFewRows; // more rows: in blocks of kFewRows
+    p.x += m0 * p.ldx;
+    p.y += m0 * p.ldy;
+    if (p.r)
+        p.r += m0 * p.ldr;
+    p.m = min(p.m - m0, kFewRows);
     f4 acc[CT][MT];
 #pragma unroll
     for (int c = 0; c < CT; c++)
@@ -450,11 +459,11 @@ int run_any(LinearParams p, hipStream_t stream)
 template <typename IO, int ACT>
 int run_linear(const LinearParams& p, hipStream_t stream)
 {
-    // the large tile where it has three rounds of CUs and more: 16000 x 2561 ->
-    // 2561 (2625 tiles) takes 631 us in it and 677 in the small one, 4000 rows
-    // (672 tiles) 177 and 178, 2000 rows (336) 118 and 101
+    // the large tile where it gives every CU one: 2561 -> 2561 at 2000 rows (336
+    // tiles) 80 us in it and 100 in the small one, 4000 rows 148 and 175; 1001 ->
+    // 777 at 1999 rows (112) 33 and 20
     const long long tiles = ((p.m + 127LL) / 128) * ((p.n + 127LL) / 128);
-    return tiles >= 768 ? run_any<IO, ACT, 128>(p, stream) : run_any<IO, ACT, 64>(p, stream);
+    return tiles >= 256 ? run_any<IO, ACT, 128>(p, stream) : run_any<IO, ACT, 64>(p, stream);
 }
 
 template <typename IO, int MT, int CT, bool WHOLE>
@@ -465,10 +474,27 @@ int run_few(const LinearParams& p, hipStream_t stream)
                                    "linear_few: dynamic LDS attribute");
     if (rc != SV2_OK)
         return rc;
-    const unsigned grid = static_cast<unsigned>((p.n + 16LL * CT - 1) / (16 * CT));
-    hipLaunchKernelGGL((linear_few_kernel<IO, MT, CT, WHOLE>), dim3(grid), dim3(64 * kFewWaves), kLds, stream, p);
+    const dim3 grid(static_cast<unsigned>((p.n + 16LL * CT - 1) / (16 * CT)), static_cast<unsigned>((p.m + kFewRows - 1) / kFewRows));
+    hipLaunchKernelGGL((linear_few_kernel<IO, MT, CT, WHOLE>), grid, dim3(64 * kFewWaves), kLds, stream, p);
     const hipError_t err = hipGetLastError();
     return err == hipSuccess ? SV2_OK : hip_error(err, "sv2_linear launch");
+}
+
+// Microseconds of the few form (MI355X): rounds of one workgroup a CU, each a
+// stream of w and x through LDS (2560 -> 2560 takes 6.5 / 11 / 16 us at 64 /
+// 128 / 256 rows: 160 / 320 / 640 workgroups, 5.5 us a round), and not faster
+// than w comes from HBM.
+double few_us(const LinearParams& p, int ct)
+{
+    const double groups = static_cast<double>((p.n + 16LL * ct - 1) / (16 * ct)) * ((p.m + kFewRows - 1) / kFewRows);
+    const double round = ct == 4 ? 2.0 + 0.0041 * p.k : 1.4 + 0.0017 * p.k;
+    return 1.5 + std::max(std::ceil(groups / 256) * round, 2e-6 * p.n * p.k / 5.0);
+}
+// Columns of a workgroup, in 16s: wide ones read x once for 64 columns and have
+// fewer workgroups (only worth it with x of more than 32 rows).
+int few_columns(const LinearParams& p)
+{
+    return p.m > 32 && few_us(p, 4) < few_us(p, 1) ? 4 : 1;
 }
 
 template <typename IO, bool WHOLE>
@@ -478,10 +504,7 @@ int run_few_rows(const LinearParams& p, hipStream_t stream)
         return run_few<IO, 1, 1, WHOLE>(p, stream);
     if (p.m <= 32)
         return run_few<IO, 2, 1, WHOLE>(p, stream);
-    // x is read once for every 16 CT columns
-    if (p.n >= 64 * 160)
-        return run_few<IO, 4, 4, WHOLE>(p, stream);
-    return run_few<IO, 4, 1, WHOLE>(p, stream);
+    return few_columns(p) == 4 ? run_few<IO, 4, 4, WHOLE>(p, stream) : run_few<IO, 4, 1, WHOLE>(p, stream);
 }
 
 template <typename IO>
@@ -559,14 +582,17 @@ try
     // pieces of 16 bytes: the rows a workgroup fetches lie within 32-bit offsets
     const bool whole = p.ldx % 8 == 0 && p.ldw % 8 == 0 && !misaligned(p.x, 16) && !misaligned(p.w, 16) &&
                        std::max(p.ldx, p.ldw) < (1LL << 31) / (2 * kFewRows);
-    if (p.m <= kFewRows)
+    const LinearOperands o{p.x, p.w, p.y, p.r, p.bias, p.ldx, p.ldw, p.ldy, p.ldr, p.m, p.n, p.k, p.act, a.dtype == SV2_BF16};
+    const bool tiles = linear_tiles_fit(o);
+    // a few blocks of 64 rows stream faster than they fill tiles (2560 -> 2560
+    // up to 384 rows, 640 -> 640 and 512 rows)
+    if (p.m <= kFewRows || (whole && tiles && p.m <= kFewMost && few_us(p, few_columns(p)) < linear_tiles_us(o)))
     {
         if (a.dtype == SV2_F16)
             return whole ? run_few_rows<HalfIO, true>(p, st) : run_few_rows<HalfIO, false>(p, st);
         return whole ? run_few_rows<BfloatIO, true>(p, st) : run_few_rows<BfloatIO, false>(p, st);
     }
-    const LinearOperands o{p.x, p.w, p.y, p.r, p.bias, p.ldx, p.ldw, p.ldy, p.ldr, p.m, p.n, p.k, p.act, a.dtype == SV2_BF16};
-    if (linear_tiles_fit(o))
+    if (tiles)
         return linear_tiles(st, o);
     return a.dtype == SV2_F16 ? run_act<HalfIO>(p, a.activation, st) : run_act<BfloatIO>(p, a.activation, st);
 }

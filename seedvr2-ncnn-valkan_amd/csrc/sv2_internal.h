@@ -218,6 +218,7 @@ struct LinearOperands
 constexpr int kGemmLinear = 3; // + sv2_activation: the tile kernel's epilogue codes from here on
 bool linear_tiles_fit(const LinearOperands& o);
 int linear_tiles(hipStream_t stream, const LinearOperands& o);
+double linear_tiles_us(const LinearOperands& o); // by the measured tile costs
 
 // fp16 y = epilogue(x W^T) for 1-64 rows on the weight-streaming kernel
 // (gemm_few.hip), the same epilogues as gemm_mfma (kGemmStore also takes an
