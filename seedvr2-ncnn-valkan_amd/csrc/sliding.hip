@@ -481,8 +481,11 @@ struct Place
 
 // Tile form: 128 rows by four waves of 32, tiles of 64 keys in two LDS
 // buffers, the next one on its way while one is worked on; one barrier a tile.
-template <typename IO, int D>
-__global__ __launch_bounds__(64 * kWaves, 2) void slide_tile_kernel(SlideParams p)
+// GROUPS = 2, for launches that give a CU one workgroup at most: a second
+// group of four waves takes every other tile for the same rows, and its sums
+// are joined to the first's in LDS.
+template <typename IO, int D, int GROUPS>
+__global__ __launch_bounds__(64 * kWaves * GROUPS, 2) void slide_tile_kernel(SlideParams p)
 {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     constexpr int kRowBytes = 2 * D;
@@ -502,28 +505,35 @@ __global__ __launch_bounds__(64 * kWaves, 2) void slide_tile_kernel(SlideParams 
     const KeyTiles<kKeys> kt(p, at.nk, p0, p1);
     const int share = (kt.count + p.splits - 1) / p.splits;
     const int t0 = min(at.split * share, kt.count);
-    const int t1 = min(t0 + share, kt.count);
+    const int nt = min(share, kt.count - t0);
+    const int steps = (nt + GROUPS - 1) / GROUPS; // of every group; its last may be empty
 
     const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % kWaves;
+    const int group = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / kWaves;
     const int row = first + wave * 32 + (lane & 31);
     Rows<IO, D> r;
     r.init(p, at.b, at.kvh, min(row, at.rows - 1), at.off, at.nk, lane);
 
     const char* kb = p.k + at.b * p.k_b + at.kvh * p.k_h;
     const char* vb = p.v + at.b * p.v_b + at.kvh * p.v_h;
-    const unsigned lds0 = static_cast<unsigned>(reinterpret_cast<size_t>(smem));
+    char* const mine = smem + group * 2 * kBuf;
+    const unsigned lds0 = static_cast<unsigned>(reinterpret_cast<size_t>(mine));
     const unsigned k_step = static_cast<unsigned>(p.k_t);
     const unsigned v_step = static_cast<unsigned>(p.v_t);
-    auto fetch = [&](int k0, int buf) {
+    auto fetch = [&](int i) {
+        const int t = GROUPS * i + group;
+        if (t >= nt)
+            return;
+        const int k0 = kt.key(t0 + t);
         const int last = at.nk - 1 - k0; // rows past the end repeat the last one
         const char* kp = kb + k0 * p.k_t;
         const char* vp = vb + k0 * p.v_t;
-        const unsigned d = lds0 + buf * kBuf;
+        const unsigned d = lds0 + (i & 1) * kBuf;
 #pragma unroll
-        for (int i = 0; i < kDma; i++)
+        for (int j = 0; j < kDma; j++)
         {
-            const int r0 = (wave * kDma + i) * kRowsPerDma;
+            const int r0 = (wave * kDma + j) * kRowsPerDma;
             const unsigned r = r0 + lane / kChunks;
             const unsigned c = lane % kChunks;
             const unsigned rr = min(static_cast<int>(r), last);
@@ -531,17 +541,17 @@ __global__ __launch_bounds__(64 * kWaves, 2) void slide_tile_kernel(SlideParams 
             dma16(vp, rr * v_step + ((c ^ value_swz<D>(r)) << 4), d + kTileBytes + r0 * kRowBytes);
         }
     };
-    if (t0 < t1)
-        fetch(kt.key(t0), 0);
-    for (int t = t0; t < t1; t++)
+    fetch(0);
+    for (int i = 0; i < steps; i++)
     {
-        const int buf = (t - t0) & 1;
         wait_vm<0>();
         bar(); // the tile is whole, and the other buffer's readers are done
-        if (t + 1 < t1)
-            fetch(kt.key(t + 1), buf ^ 1);
-        const int k0 = kt.key(t);
-        const char* st = smem + buf * kBuf;
+        fetch(i + 1);
+        const int t = GROUPS * i + group;
+        if (GROUPS > 1 && t >= nt)
+            continue;
+        const int k0 = kt.key(t0 + t);
+        const char* st = mine + (i & 1) * kBuf;
         const bool masked = is_masked(p, at.nk, p0, p1, k0, kKeys);
         f16v s[2];
         u4 w[4];
@@ -552,6 +562,45 @@ __global__ __launch_bounds__(64 * kWaves, 2) void slide_tile_kernel(SlideParams 
         r.read_values(v0, st + kTileBytes, 0);
         r.template weights<2>(s, w);
         r.template add<2>(w, v0, st + kTileBytes, k0, masked);
+    }
+    if constexpr (GROUPS > 1)
+    {
+        // the second group's registers, to the lanes that hold the same rows
+        bar();
+        float4* give = reinterpret_cast<float4*>(smem) + wave * 4 * kBlocks * 64 + lane;
+        float2* give_ml = reinterpret_cast<float2*>(smem + kWaves * 4 * kBlocks * 64 * 16) + wave * 64 + lane;
+        static_assert(kWaves * (4 * kBlocks * 64 * 16 + 64 * 8) <= GROUPS * 2 * kBuf, "the sums fit the buffers");
+        if (group == 1)
+        {
+#pragma unroll
+            for (int i = 0; i < kBlocks; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    give[(4 * i + e) * 64] = make_float4(r.o[i][4 * e], r.o[i][4 * e + 1], r.o[i][4 * e + 2], r.o[i][4 * e + 3]);
+            *give_ml = make_float2(r.m, r.l);
+        }
+        __syncthreads();
+        if (group == 1)
+            return;
+        const float2 ml = *give_ml;
+        const float m = fmaxf(r.m, ml.x);
+        const float base = m == kNegInf ? 0.f : m;
+        // a group that saw no key of a row adds nothing
+        const float ca = r.m == kNegInf ? 0.f : __builtin_amdgcn_exp2f(r.m - base);
+        const float cb = ml.x == kNegInf ? 0.f : __builtin_amdgcn_exp2f(ml.x - base);
+        r.m = m;
+        r.l = r.l * ca + ml.y * cb;
+#pragma unroll
+        for (int i = 0; i < kBlocks; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+            {
+                const float4 v = give[(4 * i + e) * 64];
+                r.o[i][4 * e] = r.o[i][4 * e] * ca + v.x * cb;
+                r.o[i][4 * e + 1] = r.o[i][4 * e + 1] * ca + v.y * cb;
+                r.o[i][4 * e + 2] = r.o[i][4 * e + 2] * ca + v.z * cb;
+                r.o[i][4 * e + 3] = r.o[i][4 * e + 3] * ca + v.w * cb;
+            }
     }
 
     const float l = partner_sum(r.l);
@@ -889,13 +938,17 @@ long long workspace_of(const SlideParams& p, int head_dim)
 template <typename IO, int D>
 int run_slide(const SlideParams& p, hipStream_t stream)
 {
-    const int lds = p.few ? FewShape<D>::kLds : 2 * 2 * kKeys * 2 * D;
-    auto kernel = p.few ? &slide_few_kernel<IO, D> : &slide_tile_kernel<IO, D>;
+    const int groups = p.blocks <= 256 ? 2 : 1; // one workgroup a CU: twice the waves
+    const int lds = p.few ? FewShape<D>::kLds : groups * 2 * 2 * kKeys * 2 * D;
+    const int threads = 64 * (p.few ? kFewWaves : kWaves * groups);
+    auto kernel = p.few         ? &slide_few_kernel<IO, D>
+                  : groups == 2 ? &slide_tile_kernel<IO, D, 2>
+                                : &slide_tile_kernel<IO, D, 1>;
     const int rc = set_dynamic_lds(reinterpret_cast<const void*>(kernel), lds, "sv2_sliding_attention: dynamic LDS attribute");
     if (rc != SV2_OK)
         return rc;
     const unsigned grid = (static_cast<unsigned>(p.blocks) + 7) / 8 * 8;
-    hipLaunchKernelGGL(kernel, dim3(grid), dim3(64 * (p.few ? kFewWaves : kWaves)), lds, stream, p);
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), lds, stream, p);
     if (p.splits > 1)
     {
         const long long rows = static_cast<long long>(p.batch) * p.heads * p.q_len;
