@@ -14,7 +14,10 @@
 //                 the order of the keys in the product's sum is free, and the
 //                 values come from LDS by transposing reads in that order.
 // P is rounded to the inputs' type (the matrix instruction takes no mixed
-// types); the sum of the weights is of the unrounded ones.
+// types), which adds as much to the output's error as its own rounding does;
+// the sum of the weights is of the unrounded ones.  Where the cache's bytes
+// are the bound (the few form) P goes in as two such numbers, the second the
+// first one's rounding error: its products cost nothing there.
 //
 // A query row here is a (position, head) pair: the heads that share a key head
 // are packed into one tile of rows, position-major, so that a tile covers few
@@ -62,6 +65,10 @@ struct HalfIO
         typedef __attribute__((ext_vector_type(2))) _Float16 h2;
         return __builtin_bit_cast(unsigned, h2{static_cast<_Float16>(lo), static_cast<_Float16>(hi)});
     }
+    static __device__ float to_float(unsigned bits)
+    {
+        return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(bits)));
+    }
 };
 struct BfloatIO
 {
@@ -77,6 +84,7 @@ struct BfloatIO
         typedef __attribute__((ext_vector_type(2))) __bf16 b2;
         return __builtin_bit_cast(unsigned, b2{static_cast<__bf16>(lo), static_cast<__bf16>(hi)});
     }
+    static __device__ float to_float(unsigned bits) { return __builtin_bit_cast(float, bits << 16); }
 };
 
 struct SlideParams
@@ -375,11 +383,12 @@ struct Rows
         for (int i = 0; i < kBlocks; i++)
             a[i] = values(vals, i, c);
     }
-    // sums += weights values (`first`: the operands of the first 16 keys); in
-    // a masked tile (from key k0 on) values that are not finite stay out of
-    // the product
+    // sums += weights values (`first`: the operands of the first 16 keys;
+    // `rest`: what the weights lack, if given); in a masked tile (from key k0
+    // on) values that are not finite stay out of the product
     template <int NB>
-    __device__ void add(const u4 (&w)[2 * NB], u4 (&first)[kBlocks], const char* vals, int k0, bool masked)
+    __device__ void add(const u4 (&w)[2 * NB], u4 (&first)[kBlocks], const char* vals, int k0, bool masked,
+                        const u4* rest = nullptr)
     {
         u4 next[kBlocks];
 #pragma unroll
@@ -405,6 +414,10 @@ struct Rows
 #pragma unroll
             for (int i = 0; i < kBlocks; i++)
                 o[i] = IO::mfma(a[i], w[c], o[i]);
+            if (rest)
+#pragma unroll
+                for (int i = 0; i < kBlocks; i++)
+                    o[i] = IO::mfma(a[i], rest[c], o[i]);
         }
     }
     // Takes the values that are +Inf, -Inf or NaN out of an operand (of 16
@@ -722,7 +735,15 @@ __global__ __launch_bounds__(64 * kFewWaves) void slide_few_kernel(SlideParams p
         u4 v0[Rows<IO, D>::kBlocks];
         r.read_values(v0, st + S::kTileBytes, 0);
         r.template weights<1>(s, w);
-        r.template add<1>(w, v0, st + S::kTileBytes, k0, masked);
+        // their rounding errors
+        u4 rest[2];
+#pragma unroll
+        for (int c = 0; c < 2; c++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                rest[c][e] = IO::pack(s[0][8 * c + 2 * e] - IO::to_float(w[c][e] & 0xffffu),
+                                      s[0][8 * c + 2 * e + 1] - IO::to_float(w[c][e] >> 16));
+        r.template add<1>(w, v0, st + S::kTileBytes, k0, masked, rest);
     }
 
     // the waves' sums, relative to the largest maximum of a row
