@@ -596,12 +596,12 @@ __global__ __launch_bounds__(kRowThreads) void norm_apply_kernel(NormArgs p)
     }
 }
 
-// The rows form's runs: enough workgroups for 256 CUs, at least 16 KB each.
+// The rows form's runs: enough workgroups for 256 CUs, at least 32 KB each.
 void plan_rows(NormArgs* p, int images, int bytes)
 {
     const long long row_bytes = static_cast<long long>(p->channels) * bytes;
     const long long want = (static_cast<long long>(images) * p->rows + 2047) / 2048;
-    const long long least = std::max(1LL, 16384 / row_bytes);
+    const long long least = std::max(1LL, 32768 / row_bytes);
     p->chunk_rows = static_cast<int>(std::min<long long>(p->rows, std::max(want, least)));
     p->chunks = (p->rows + p->chunk_rows - 1) / p->chunk_rows;
 }
