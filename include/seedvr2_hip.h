@@ -679,17 +679,11 @@ typedef struct sv2_linear_args {
     int64_t residual_stride;
     void* y;
     int64_t y_stride;
-    void* workspace; /* device, sv2_linear_workspace() bytes, 16-byte aligned; not shared by calls that may overlap */
-    size_t workspace_bytes;
 } sv2_linear_args;
 
-/* Host.  Device workspace bytes of a call with these sizes (its pointers and
- * strides do not matter), or a negative error code. */
-int64_t sv2_linear_workspace(const sv2_linear_args* args);
-
-/* Device.  The product above; any sizes, strides and element alignment.
- * Operands that are 16-byte aligned with row strides of a multiple of 8
- * elements run on the faster kernels. */
+/* Device.  The product above; any sizes, strides and element alignment, no
+ * workspace.  Operands that are 16-byte aligned with row strides of a multiple
+ * of 8 elements run on the faster kernels.  Results do not depend on timing. */
 int sv2_linear(const sv2_linear_args* args, void* stream);
 
 /* ---- Euler sampler (src/model/sampler.h:18-78) and the latent preparation

@@ -600,7 +600,8 @@ __global__ __launch_bounds__(kRowThreads) void norm_apply_kernel(NormArgs p)
 void plan_rows(NormArgs* p, int images, int bytes)
 {
     const long long row_bytes = static_cast<long long>(p->channels) * bytes;
-    const long long want = (static_cast<long long>(images) * p->rows + 2047) / 2048;
+    // kMaxChunks runs in all, so no image has more
+    const long long want = (static_cast<long long>(images) * p->rows + kMaxChunks - 1) / kMaxChunks;
     const long long least = std::max(1LL, 32768 / row_bytes);
     p->chunk_rows = static_cast<int>(std::min<long long>(p->rows, std::max(want, least)));
     p->chunks = (p->rows + p->chunk_rows - 1) / p->chunk_rows;

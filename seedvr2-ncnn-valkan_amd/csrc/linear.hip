@@ -519,15 +519,15 @@ int run_act(const LinearParams& p, int activation, hipStream_t stream)
     }
 }
 
-int check_linear(const sv2_linear_args* a, const char* what)
+int check_linear(const sv2_linear_args* a)
 {
-    auto bad = [&](const char* why) { return set_error(SV2_EINVAL, std::string(what) + ": " + why); };
+    auto bad = [&](const char* why) { return set_error(SV2_EINVAL, std::string("sv2_linear: ") + why); };
     if (!a)
         return bad("null arguments");
     if (a->rows < 0 || a->in <= 0 || a->out < 0)
         return bad("negative sizes");
     if (a->dtype != SV2_F16 && a->dtype != SV2_BF16)
-        return set_error(a->dtype == SV2_F32 ? SV2_EUNSUPPORTED : SV2_EINVAL, std::string(what) + ": dtype must be SV2_F16 or SV2_BF16");
+        return set_error(a->dtype == SV2_F32 ? SV2_EUNSUPPORTED : SV2_EINVAL, "sv2_linear: dtype must be SV2_F16 or SV2_BF16");
     if (a->activation < SV2_ACT_NONE || a->activation > SV2_ACT_GELU_TANH)
         return bad("unknown activation");
     if (a->x_stride < a->in || a->w_stride < a->in || a->y_stride < a->out || (a->residual && a->residual_stride < a->out))
@@ -538,22 +538,11 @@ int check_linear(const sv2_linear_args* a, const char* what)
 } // namespace
 } // namespace sv2
 
-extern "C" int64_t sv2_linear_workspace(const sv2_linear_args* args)
-try
-{
-    const int rc = sv2::check_linear(args, "sv2_linear_workspace");
-    return rc != SV2_OK ? rc : 0;
-}
-catch (...)
-{
-    return sv2::caught_exception("sv2_linear_workspace");
-}
-
 extern "C" int sv2_linear(const sv2_linear_args* args, void* stream)
 try
 {
     using namespace sv2;
-    const int rc = check_linear(args, "sv2_linear");
+    const int rc = check_linear(args);
     if (rc != SV2_OK)
         return rc;
     const sv2_linear_args& a = *args;

@@ -312,13 +312,14 @@ struct Rows
         if (k0 >= sinks)
         {
             // lo_key <= j <= hi_key in one comparison (hi_key < lo_key: nothing)
-            const unsigned range = hi_key >= lo_key ? static_cast<unsigned>(hi_key - lo_key) : 0u;
-            const int d = hi_key >= lo_key ? k0 - lo_key : -(1 << 30);
+            const bool any = hi_key >= lo_key;
+            const unsigned range = any ? static_cast<unsigned>(hi_key) - static_cast<unsigned>(lo_key) : 0u;
+            const unsigned d = any ? static_cast<unsigned>(key_of(k0, 0, 0)) - static_cast<unsigned>(lo_key) : 1u << 30;
 #pragma unroll
             for (int i = 0; i < NB; i++)
 #pragma unroll
                 for (int e = 0; e < 16; e++)
-                    s[i][e] = static_cast<unsigned>(key_of(d, i, e)) <= range ? s[i][e] : kNegInf;
+                    s[i][e] = d + (32u * i + 8u * (e >> 2) + (e & 3)) <= range ? s[i][e] : kNegInf;
             return;
         }
 #pragma unroll
@@ -634,14 +635,17 @@ __global__ __launch_bounds__(64 * kWaves * GROUPS, 2) void slide_tile_kernel(Sli
             p.part_ml[part] = make_float2(r.m, l);
         return;
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float inv = 1.f / l;
     char* dst = p.out + at.b * p.o_b + r.qi * p.o_t + r.head * p.o_h + 8 * r.half;
 #pragma unroll
     for (int i = 0; i < kBlocks; i++)
 #pragma unroll
         for (int e = 0; e < 4; e++)
-            *reinterpret_cast<u2*>(dst + 64 * i + 16 * e) =
-                u2{IO::pack(r.o[i][4 * e] * inv, r.o[i][4 * e + 1] * inv), IO::pack(r.o[i][4 * e + 2] * inv, r.o[i][4 * e + 3] * inv)};
+        {
+            const u2 v = {IO::pack(r.o[i][4 * e] * inv, r.o[i][4 * e + 1] * inv),
+                          IO::pack(r.o[i][4 * e + 2] * inv, r.o[i][4 * e + 3] * inv)};
+            *reinterpret_cast<u2*>(dst + 64 * i + 16 * e) = l == 0.f ? u2{0u, 0u} : v; // no key: 0
+        }
     if (p.lse && r.half == 0)
         p.lse[to] = l == 0.f ? kNegInf : r.m * kLn2 + logf(l);
 }
@@ -801,9 +805,9 @@ __global__ __launch_bounds__(64 * kFewWaves) void slide_few_kernel(SlideParams p
                 p.part_ml[to_part] = make_float2(m, total);
             continue;
         }
-        const float inv = total == 0.f ? 0.f : 1.f / total;
+        const float inv = 1.f / total;
         *reinterpret_cast<u2*>(p.out + at.b * p.o_b + qi * p.o_t + head * p.o_h + 2 * d) =
-            u2{IO::pack(v.x * inv, v.y * inv), IO::pack(v.z * inv, v.w * inv)};
+            total == 0.f ? u2{0u, 0u} : u2{IO::pack(v.x * inv, v.y * inv), IO::pack(v.z * inv, v.w * inv)};
         if (p.lse && d == 0)
             p.lse[to] = total == 0.f ? kNegInf : m * kLn2 + logf(total);
     }
@@ -878,6 +882,8 @@ __global__ __launch_bounds__(32 * kTeams) void slide_join_kernel(SlideParams p, 
         l = l * a + c * ml.y;
         o = o * a + c * s_sum[team + t][lane];
     }
+    if (l == 0.f)
+        o = fe{}; // no key
     const float inv = l == 0.f ? 0.f : 1.f / l;
     char* dst = p.out + b * p.o_b + qi * p.o_t + head * p.o_h + 2 * kE * lane;
     if constexpr (kE == 4)

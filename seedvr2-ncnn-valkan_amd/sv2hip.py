@@ -86,7 +86,6 @@ EXPORTS = [
     "sv2_sliding_attention",
     "sv2_group_norm_workspace",
     "sv2_group_norm",
-    "sv2_linear_workspace",
     "sv2_linear",
     "sv2_euler_timesteps",
     "sv2_condition_ratio",
@@ -173,8 +172,6 @@ class LinearArgs(ctypes.Structure):
         ("residual_stride", ctypes.c_int64),
         ("y", ctypes.c_void_p),
         ("y_stride", ctypes.c_int64),
-        ("workspace", ctypes.c_void_p),
-        ("workspace_bytes", ctypes.c_size_t),
     ]
 
 
@@ -389,8 +386,6 @@ def load() -> ctypes.CDLL:
     lib.sv2_group_norm.argtypes = [vp, i64, i64, vp, i64, i64, i, i, i, i, i, ctypes.c_float, vp, vp, i, vp,
                                    ctypes.c_size_t, vp]
     lib.sv2_group_norm.restype = i
-    lib.sv2_linear_workspace.argtypes = [ctypes.POINTER(LinearArgs)]
-    lib.sv2_linear_workspace.restype = ctypes.c_int64
     lib.sv2_linear.argtypes = [ctypes.POINTER(LinearArgs), vp]
     lib.sv2_linear.restype = i
     lib.sv2_euler_timesteps.argtypes = [i, vp]
@@ -1244,7 +1239,8 @@ def sliding_attention(q, k, v, out, *, left, right=0, sinks=0, scale=None, q_len
                         d ** -0.5 if scale is None else scale,
                         *_need("q", q, dtype, shape, dev), *_need("k", k, dtype, cache, dev),
                         *_need("v", v, dtype, cache, dev), *_need("out", out, dtype, shape, dev),
-                        _dense_ptr("q_lens", q_lens, torch.int32, (b,), dev), _dense_ptr("kv_lens", kv_lens, torch.int32, (b,), dev),
+                        _dense_ptr("q_lens", q_lens, torch.int32, (b,), dev),
+                        _dense_ptr("kv_lens", kv_lens, torch.int32, (b,), dev),
                         _dense_ptr("lse", lse, torch.float32, (b, h, nq), dev))
     lib = load()
     ref = ctypes.byref(a)
@@ -1283,7 +1279,7 @@ def group_norm(x, y, groups, *, gamma=None, beta=None, eps=1e-5, activation=ACT_
     return y
 
 
-def linear(x, w, y, *, bias=None, activation=ACT_NONE, residual=None, workspace=None, stream=None):
+def linear(x, w, y, *, bias=None, activation=ACT_NONE, residual=None, stream=None):
     """y = act(x W^T + bias) + residual (sv2_linear): x [rows, in], w [out, in],
     y and residual [rows, out], all fp16 or all bf16 with contiguous rows; bias
     fp32 [out].  y may be the residual."""
@@ -1301,16 +1297,7 @@ def linear(x, w, y, *, bias=None, activation=ACT_NONE, residual=None, workspace=
                    None if residual is None else residual.data_ptr(), 0 if residual is None else _row_step(residual),
                    y.data_ptr(), _row_step(y))
     lib = load()
-    ref = ctypes.byref(a)
-    need = lib.sv2_linear_workspace(ref)
-    if need < 0:
-        check(need, "sv2_linear_workspace")
-
-    def call(ptr, size, raw):
-        a.workspace, a.workspace_bytes = ptr, size
-        return lib.sv2_linear(ref, raw)
-
-    check(_enqueue(call, x, workspace, need, stream), "sv2_linear")
+    check(_enqueue(lambda ptr, size, raw: lib.sv2_linear(ctypes.byref(a), raw), x, None, 0, stream), "sv2_linear")
     return y
 
 

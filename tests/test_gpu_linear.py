@@ -56,6 +56,25 @@ def test_sizes(hip, device, m, k, n, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("m,k,n", [
+    (1100, 192, 1288), (1500, 264, 776), (3000, 520, 1288), (2600, 1000, 2568), (8200, 64, 264), (4100, 136, 2050),
+    (2049, 2560, 640), (1300, 1096, 513),
+    (100, 1280, 640), (500, 640, 640), (130, 2560, 2560), (257, 1000, 1024), (65, 640, 10250),
+])
+@pytest.mark.parametrize("act,residual", [(0, True), (3, False)])
+def test_forms_of_many_rows(hip, device, m, k, n, act, residual, dtype):
+    """Whole tiles and cut ones of each size, K with and without a rest, and
+    rows streamed in blocks of 64."""
+    check(hip, device, m, k, n, TD[dtype], act=act, residual=residual)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("m,k,n", [(2100, 133, 2051), (3000, 70, 3001)])
+def test_large_tiles_of_any_alignment(hip, device, m, k, n, dtype):
+    check(hip, device, m, k, n, TD[dtype], act=1, pad=1)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("m,k,n", [(1, 320, 192), (40, 320, 192), (600, 320, 256)])
 @pytest.mark.parametrize("act", [0, 1, 2, 3])
 @pytest.mark.parametrize("bias,residual", [(False, False), (True, False), (False, True), (True, True)])
@@ -70,12 +89,11 @@ def test_strides_and_alignment(hip, device, m, k, n, pad, shift, dtype):
     check(hip, device, m, k, n, TD[dtype], act=3, pad=pad, shift=shift)
 
 
-@pytest.mark.parametrize("m", [1, 50, 700])
+@pytest.mark.parametrize("m", [1, 50, 700, 5000])
 def test_in_place_residual_and_repeatable(hip, device, m):
-    x, w, b, r, y = check(hip, device, m, 512, 256, torch.bfloat16, act=2)
+    x, w, b, r, y = check(hip, device, m, 512, 250, torch.bfloat16, act=2, pad=6)
     z = r.clone()
-    ws = torch.full((64 << 20,), 0xFF, dtype=torch.uint8, device=device)
-    hip.linear(x, w, z, bias=b, activation=2, residual=z, workspace=ws)
+    hip.linear(x, w, z, bias=b, activation=2, residual=z)
     torch.cuda.synchronize()
     assert torch.equal(z, y)
 
@@ -102,13 +120,12 @@ def test_streams_and_graph(hip, device, m, k, n):
     y = torch.empty((m, n), dtype=torch.float16, device=device)
     s = torch.cuda.Stream()
     s.wait_stream(torch.cuda.current_stream())
-    ws = torch.empty(64 << 20, dtype=torch.uint8, device=device)
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.stream(s):
-        hip.linear(x, w, y, workspace=ws)
+        hip.linear(x, w, y)
         torch.cuda.synchronize()
         with torch.cuda.graph(graph, stream=s):
-            hip.linear(x, w, y, workspace=ws)
+            hip.linear(x, w, y)
     for _ in range(3):
         x.normal_()
         y.zero_()

@@ -80,6 +80,23 @@ def test_lengths_and_windows(hip, device, b, nq, nk, h, g, d, left, right, sinks
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("b,nq,nk,h,g,left,right,sinks", [
+    (3, 1000, 1000, 12, 12, 200, 0, 20),   # more row tiles than CUs
+    (2, 700, 900, 40, 10, 300, 50, 3),
+    (1, 32, 6000, 2, 2, 6000, 0, 0),       # 32 rows a key head, many splits
+    (1, 33, 6000, 2, 2, 6000, 0, 0),       # one more
+    (2, 8, 9000, 8, 2, 8000, 7, 100),      # eight tokens of four heads
+    (1, 5, 300, 30, 5, 299, 0, 0),         # thirty rows
+    (20, 2, 500, 16, 16, 100, 0, 64),      # few splits of many heads
+    (1, 129, 40000, 1, 1, 39000, 0, 11),   # two row tiles, many splits
+])
+def test_forms(hip, device, b, nq, nk, h, g, d, left, right, sinks, dtype):
+    q, k, v = make(device, b, nq, nk, h, g, d, TD[dtype], seed=nq)
+    check(hip, q, k, v, left, right, sinks)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("layout", ["bhtd", "padded"])
 def test_layouts(hip, device, layout, dtype):
     q, k, v = make(device, 2, 50, 140, 4, 2, 128, TD[dtype], layout=layout)
@@ -128,6 +145,18 @@ def test_values_that_are_not_finite(hip, device, nq, h, g, d, dtype):
     check(hip, q, k, v, left, 0, sinks)
 
 
+@pytest.mark.parametrize("nq,h", [(40, 2), (700, 40)])
+def test_values_that_are_not_finite_in_every_tile(hip, device, nq, h):
+    """Windows so narrow that every tile is masked, with a value of each kind
+    every few keys."""
+    q, k, v = make(device, 1, nq, nq + 300, h, h, 128, torch.bfloat16)
+    v[:, 5::67, :, 3] = math.inf
+    v[:, 9::71, :, 3] = -math.inf
+    v[:, 40::97, :, 60] = math.nan
+    v[:, 50::61] = math.inf
+    check(hip, q, k, v, 20, 0, 2)
+
+
 @pytest.mark.parametrize("nq", [1, 40])
 def test_scores_that_are_not_finite(hip, device, nq):
     """A row whose only visible scores are -Inf counts as empty; +Inf and NaN
@@ -137,6 +166,9 @@ def test_scores_that_are_not_finite(hip, device, nq):
     v = torch.ones_like(k)
     out, lse = run(hip, q, k, v, 1000, 0, 0)
     assert (out == 0).all() and (lse == -math.inf).all()
+    v[0, 3] = math.inf
+    assert (run(hip, q, k, v, 1000, 0, 0)[0] == 0).all()
+    v[0, 3] = 1.0
     k[0, 3] = math.inf
     out, lse = run(hip, q, k, v, 1000, 0, 0)
     assert torch.isnan(out).all() and torch.isnan(lse).all()
