@@ -551,7 +551,7 @@ __global__ __launch_bounds__(kJoinThreads) void norm_join_kernel(NormArgs p)
 template <typename T, int V, int ACT>
 __global__ __launch_bounds__(kRowThreads) void norm_apply_kernel(NormArgs p)
 {
-    constexpr int kHeld = V == 1 ? 16 : 8;
+    constexpr int kHeld = 4;
     // backwards: what the statistics read last may still be in the last-level
     // cache
     const int block = gridDim.x - 1 - blockIdx.x;
@@ -566,32 +566,57 @@ __global__ __launch_bounds__(kRowThreads) void norm_apply_kernel(NormArgs p)
         const int col = k.rounds > 1 ? round * kRowThreads + threadIdx.x : threadIdx.x - r0 * k.nc;
         if (r0 >= k.lanes || col >= k.nc)
             continue;
-        Affine<V> f;
-        f.load(p.gamma, p.beta, col * V);
-        f.scale([&](int e) { return stat[(col * V + e) / p.width]; });
         const int mine = Share(rows, k.lanes).of(r0);
         long long xi = image * p.x_image + static_cast<long long>(first + r0) * p.x_row + col * V;
         long long yi = image * p.y_image + static_cast<long long>(first + r0) * p.y_row + col * V;
         const long long xs = k.lanes * p.x_row;
         const long long ys = k.lanes * p.y_row;
-        for (int done = 0; done < mine; done += kHeld)
+        // the next rows are on their way while these are normalised, the first
+        // while the factors are
+        Piece<T, V> ahead[kHeld];
+        if (kHeld <= mine)
+#pragma unroll
+            for (int i = 0; i < kHeld; i++)
+                ahead[i].load(p.x, xi + i * xs);
+        Affine<V> f;
+        f.load(p.gamma, p.beta, col * V);
+        if (p.unit == V)
+        {
+            const float2 one = stat[col * V / p.width];
+            f.scale([&](int) { return one; });
+        }
+        else
+            f.scale([&](int e) { return stat[(col * V + e) / p.width]; });
+        auto finish = [&](const Piece<T, V>& h, long long to) {
+            float x[V];
+            h.get(x);
+            f.template apply<ACT, std::is_same_v<T, F32>>(x);
+            Piece<T, V>::store(p.y, to, x);
+        };
+        int done = 0;
+        for (; done + kHeld <= mine; done += kHeld)
         {
             Piece<T, V> h[kHeld];
 #pragma unroll
             for (int i = 0; i < kHeld; i++)
-                if (done + i < mine)
-                    h[i].load(p.x, xi + i * xs);
+                h[i] = ahead[i];
+            xi += kHeld * xs;
+            if (done + 2 * kHeld <= mine)
+#pragma unroll
+                for (int i = 0; i < kHeld; i++)
+                    ahead[i].load(p.x, xi + i * xs);
 #pragma unroll
             for (int i = 0; i < kHeld; i++)
-                if (done + i < mine)
-                {
-                    float x[V];
-                    h[i].get(x);
-                    f.template apply<ACT, std::is_same_v<T, F32>>(x);
-                    Piece<T, V>::store(p.y, yi + i * ys, x);
-                }
-            xi += kHeld * xs;
+                finish(h[i], yi + i * ys);
             yi += kHeld * ys;
+        }
+        for (; done < mine; done++)
+        {
+            Piece<T, V> h;
+            h.load(p.x, xi);
+            finish(h, yi);
+            xi += xs;
+            yi += ys;
         }
     }
 }
