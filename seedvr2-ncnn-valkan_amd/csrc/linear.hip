@@ -158,7 +158,7 @@ __device__ inline void wait_vm()
 
 constexpr int kFewWaves = 4;
 constexpr int kFewRows = 64;
-constexpr int kFewMost = 1024; // rows the few form is weighed for
+constexpr int kFewMost = 1 << 20; // rows the few form is weighed for (its grid holds 65535 blocks of rows)
 
 // The few form's LDS: a ring of slots of 16 CT rows of w and 16 MT rows of x,
 // 128 bytes each, per wave; 16-byte chunk c of row r sits in slot c ^ (r & 7),
@@ -308,7 +308,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_few_kernel(LinearParams
 }
 
 // Any form: TILE x TILE outputs by 4 waves, K in steps of 64 through registers
-// (three steps ahead of their use) into two LDS buffers.  16-byte loads at any
+// (kHeld steps ahead) into two LDS buffers.  16-byte loads at any
 // element alignment; only the last step looks at K's end.
 template <int TILE>
 struct AnyShape
@@ -317,10 +317,13 @@ struct AnyShape
     static constexpr int kOperand = TILE * kPitch;
     static constexpr int kLds = 2 * 2 * kOperand;
     static constexpr int kPieces = TILE * 8 / 256; // 16-byte pieces of an operand per thread and step
+    // steps held in registers: the small tiles' launches have few waves a CU
+    // to hide the loads' latency
+    static constexpr int kHeld = TILE == 128 ? 2 : 5;
 };
 
 template <typename IO, int ACT, int TILE>
-__global__ __launch_bounds__(256, TILE == 128 ? 2 : 4) void linear_any_kernel(LinearParams p)
+__global__ __launch_bounds__(256, TILE == 128 ? 2 : 3) void linear_any_kernel(LinearParams p)
 {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     using S = AnyShape<TILE>;
@@ -410,25 +413,30 @@ __global__ __launch_bounds__(256, TILE == 128 ? 2 : 4) void linear_any_kernel(Li
                     acc[t][u] = IO::mfma(a[t], b[u], acc[t][u]);
         }
     };
-    // step s: the next one's registers go to LDS, and are loaded for step s + 3
-    auto step = [&](Held& h, int s) {
-        if (s + 1 < steps)
-            put(h, s + 1);
-        load(h, s + 3);
-        multiply(s);
-        __syncthreads();
-    };
-    Held even, odd;
-    load(even, 0);
-    load(odd, 1);
-    put(even, 0);
-    load(even, 2);
+    // step s: the next one's registers go to LDS and are loaded again, for the
+    // step kHeld further
+    Held held[S::kHeld];
+#pragma unroll
+    for (int i = 0; i < S::kHeld; i++)
+        load(held[i], i);
+    put(held[0], 0);
+    load(held[0], S::kHeld);
     __syncthreads();
-    for (int s = 0; s < steps; s += 2)
+    for (int s0 = 0; s0 < steps; s0 += S::kHeld)
     {
-        step(odd, s);
-        if (s + 1 < steps)
-            step(even, s + 1);
+#pragma unroll
+        for (int u = 0; u < S::kHeld; u++)
+        {
+            const int s = s0 + u;
+            if (s >= steps)
+                break;
+            Held& h = held[(u + 1) % S::kHeld];
+            if (s + 1 < steps)
+                put(h, s + 1);
+            load(h, s + 1 + S::kHeld);
+            multiply(s);
+            __syncthreads();
+        }
     }
 #pragma unroll
     for (int t = 0; t < kT; t++)
@@ -483,12 +491,15 @@ int run_few(const LinearParams& p, hipStream_t stream)
 // Microseconds of the few form (MI355X): rounds of one workgroup a CU, each a
 // stream of w and x through LDS (2560 -> 2560 takes 6.5 / 11 / 16 us at 64 /
 // 128 / 256 rows: 160 / 320 / 640 workgroups, 5.5 us a round), and not faster
-// than w comes from HBM.
+// than w comes from HBM and an x past an XCD's 4 MB of L2 comes once for every
+// 16 CT columns (4538 x 5312 -> 96: 290 MB and 43 us in 16s, 97 MB in 64s).
 double few_us(const LinearParams& p, int ct)
 {
     const double groups = static_cast<double>((p.n + 16LL * ct - 1) / (16 * ct)) * ((p.m + kFewRows - 1) / kFewRows);
     const double round = ct == 4 ? 2.0 + 0.0041 * p.k : 1.4 + 0.0017 * p.k;
-    return 1.5 + std::max(std::ceil(groups / 256) * round, 2e-6 * p.n * p.k / 5.0);
+    const double x_bytes = 2.0 * p.m * p.k;
+    const double x_us = x_bytes > (4 << 20) ? 1e-6 * x_bytes * ((p.n + 16LL * ct - 1) / (16 * ct)) / 7.0 : 0.0;
+    return 1.5 + std::max({std::ceil(groups / 256) * round, 2e-6 * p.n * p.k / 5.0, x_us});
 }
 // Columns of a workgroup, in 16s: wide ones read x once for 64 columns and have
 // fewer workgroups (only worth it with x of more than 32 rows).
