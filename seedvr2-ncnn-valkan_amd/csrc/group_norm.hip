@@ -220,7 +220,7 @@ struct Share
     __device__ int of(int r) const { return each + (r < more ? 1 : 0); }
 };
 
-// e / d for 0 <= e < 2^21 (pieces in LDS) and inv = 1 / d: the half keeps the
+// e / d for 0 <= e < 2^21 (threads, channels, pieces in LDS) and inv = 1 / d: the half keeps the
 // quotient's rounding errors, 2^-22 of it, from reaching a whole number.
 __device__ inline int quick_div(int e, float inv)
 {
@@ -280,7 +280,7 @@ __global__ __launch_bounds__(kSlabThreads) void norm_slab_kernel(NormArgs p)
     const int sc = ng * p.width;     // channels of this slab, a multiple of V
     const int nc = sc / V;
     const int lanes = blockDim.x / nc;
-    const int r0 = threadIdx.x / nc;
+    const int r0 = quick_div(threadIdx.x, 1.f / static_cast<float>(nc));
     const int c = (threadIdx.x - r0 * nc) * V;
     const bool active = r0 < lanes;
     const Share share(p.rows, lanes);
@@ -348,7 +348,14 @@ __global__ __launch_bounds__(kSlabThreads) void norm_slab_kernel(NormArgs p)
     __syncthreads();
     if (!active)
         return;
-    f.scale([&](int e) { return s_stat[(c + e) / p.width]; });
+    const float inv_width = 1.f / static_cast<float>(p.width);
+    if (unit == V)
+    {
+        const float2 one = s_stat[quick_div(c, inv_width)];
+        f.scale([&](int) { return one; });
+    }
+    else
+        f.scale([&](int e) { return s_stat[quick_div(c + e, inv_width)]; });
     const long long yi = image * p.y_image + c_base + c;
 #pragma unroll
     for (int k = 0; k < KEEP; k++)
@@ -393,7 +400,7 @@ __global__ __launch_bounds__(kRowThreads, 4) void norm_stats_kernel(NormArgs p)
     float2* s_piece = reinterpret_cast<float2*>(smem); // [row lane][span of unit channels]
     for (int round = 0; round < k.rounds; round++)
     {
-        const int r0 = k.rounds > 1 ? 0 : threadIdx.x / k.nc;
+        const int r0 = k.rounds > 1 ? 0 : quick_div(threadIdx.x, 1.f / static_cast<float>(k.nc));
         const int col = k.rounds > 1 ? round * kRowThreads + threadIdx.x : threadIdx.x - r0 * k.nc;
         if (r0 >= k.lanes || col >= k.nc)
             continue;
@@ -560,9 +567,10 @@ __global__ __launch_bounds__(kRowThreads) void norm_apply_kernel(NormArgs p)
     const int rows = min(p.chunk_rows, p.rows - first);
     const Columns k = columns<V>(p.channels);
     const float2* stat = p.stat + static_cast<long long>(image) * p.groups;
+    const float inv_width = 1.f / static_cast<float>(p.width);
     for (int round = 0; round < k.rounds; round++)
     {
-        const int r0 = k.rounds > 1 ? 0 : threadIdx.x / k.nc;
+        const int r0 = k.rounds > 1 ? 0 : quick_div(threadIdx.x, 1.f / static_cast<float>(k.nc));
         const int col = k.rounds > 1 ? round * kRowThreads + threadIdx.x : threadIdx.x - r0 * k.nc;
         if (r0 >= k.lanes || col >= k.nc)
             continue;
@@ -582,11 +590,11 @@ __global__ __launch_bounds__(kRowThreads) void norm_apply_kernel(NormArgs p)
         f.load(p.gamma, p.beta, col * V);
         if (p.unit == V)
         {
-            const float2 one = stat[col * V / p.width];
+            const float2 one = stat[quick_div(col * V, inv_width)];
             f.scale([&](int) { return one; });
         }
         else
-            f.scale([&](int e) { return stat[(col * V + e) / p.width]; });
+            f.scale([&](int e) { return stat[quick_div(col * V + e, inv_width)]; });
         auto finish = [&](const Piece<T, V>& h, long long to) {
             float x[V];
             h.get(x);
