@@ -640,8 +640,9 @@ typedef struct sv2_sliding_attn_args {
 int64_t sv2_sliding_attention_workspace(const sv2_sliding_attn_args* args);
 
 /* Device.  The attention above.  q, k, v, out and the workspace must be
- * 16-byte aligned and every stride a multiple of 8 elements (SV2_EINVAL; the
- * stride of a dimension of one element is not read); token strides of k and v up to 2^24 elements, head_dim 64 or 128
+ * 16-byte aligned and every stride a multiple of 8 elements, out's not 0
+ * (SV2_EINVAL; the stride of a dimension of one element is not read); token
+ * strides of k and v up to 2^24 elements, head_dim 64 or 128
  * (SV2_EUNSUPPORTED).  Results do not depend on timing. */
 int sv2_sliding_attention(const sv2_sliding_attn_args* args, void* stream);
 
@@ -654,7 +655,7 @@ int64_t sv2_group_norm_workspace(int dtype, int images, int rows, int channels, 
  * mean and biased variance per image and group of channels / groups
  * consecutive channels, over all its rows.  x, y of dtype (fp32, fp16, bf16);
  * statistics and gamma, beta (fp32 [channels], NULL: 1 and 0) in fp32.  y may
- * be x (with the same strides).  Any alignment and strides; 16-byte aligned
+ * be x with the same strides (others: SV2_EINVAL).  Any alignment and strides; 16-byte aligned
  * tensors with strides and channels in multiples of 16 bytes are several times
  * as fast.  Row strides are at least `channels`; more than 8192 channels give
  * SV2_EUNSUPPORTED.  Calls that share a workspace must not overlap. */
@@ -665,9 +666,10 @@ int sv2_group_norm(const void* x, int64_t x_image_stride, int64_t x_row_stride, 
 
 /* y [rows, out] = act(x [rows, in] W^T + bias) + residual, W [out, in]; x, W,
  * y and residual of dtype, sums and bias in fp32, one rounding at the end.
- * bias and residual may be NULL; y may be the residual (with its stride). */
+ * bias and residual may be NULL; y may be the residual with its stride
+ * (another: SV2_EINVAL). */
 typedef struct sv2_linear_args {
-    int rows, in, out;
+    int rows, in, out; /* in at least 1 */
     int dtype;      /* SV2_F16 or SV2_BF16 (fp32 products: sv2_inner_product_f32) */
     int activation; /* sv2_activation */
     const void* x;

@@ -805,6 +805,8 @@ try
     if (x_row_stride < channels || y_row_stride < channels ||
         (images > 1 && (x_image_stride < 0 || y_image_stride < channels)))
         return set_error(SV2_EINVAL, "sv2_group_norm: a stride below the channel count");
+    if (x == y && ((rows > 1 && x_row_stride != y_row_stride) || (images > 1 && x_image_stride != y_image_stride)))
+        return set_error(SV2_EINVAL, "sv2_group_norm: y is x with other strides");
     NormArgs p{};
     p.x = x;
     p.y = y;

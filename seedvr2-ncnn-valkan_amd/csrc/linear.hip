@@ -545,13 +545,15 @@ int check_linear(const sv2_linear_args* a)
     if (!a)
         return bad("null arguments");
     if (a->rows < 0 || a->in <= 0 || a->out < 0)
-        return bad("negative sizes");
+        return bad("negative rows or out, or in below 1");
     if (a->dtype != SV2_F16 && a->dtype != SV2_BF16)
         return set_error(a->dtype == SV2_F32 ? SV2_EUNSUPPORTED : SV2_EINVAL, "sv2_linear: dtype must be SV2_F16 or SV2_BF16");
     if (a->activation < SV2_ACT_NONE || a->activation > SV2_ACT_GELU_TANH)
         return bad("unknown activation");
     if (a->x_stride < a->in || a->w_stride < a->in || a->y_stride < a->out || (a->residual && a->residual_stride < a->out))
         return bad("a row stride below the row's length");
+    if (a->rows > 1 && a->residual && a->residual == a->y && a->residual_stride != a->y_stride)
+        return bad("the residual is y with another stride");
     return SV2_OK;
 }
 

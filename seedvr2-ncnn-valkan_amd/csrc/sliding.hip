@@ -66,7 +66,6 @@ typedef __attribute__((ext_vector_type(2))) unsigned u2;
 
 constexpr float kNegInf = -__builtin_inff();
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 
 struct HalfIO
 {
@@ -117,8 +116,8 @@ struct SlideParams
     const int32_t* kv_lens;
     float* lse;
     float* part;    // splits > 1: sums [split][batch][heads][q_len][head_dim]
-    float2* part_ml; // maxima (scaled, base 2) and sums of weights [split][batch][heads][q_len]
-    float scale2;   // scale * log2(e)
+    float2* part_ml; // maxima (unscaled) and sums of weights [split][batch][heads][q_len]
+    float scale, scale2; // scale2 = scale * log2(e)
     int batch, q_len, kv_len, heads, kv_heads, group;
     int left, right, sinks;
     int few, row_tiles, splits, blocks;
@@ -238,6 +237,12 @@ __device__ inline unsigned value_swz(unsigned r)
 // up to 2^8, far inside both types.
 constexpr float kRise = 8.f;
 
+// Scores (times scale2) up to here are brought down to the maximum by one
+// fused product: its rounding of the maximum moves a row's weights by 2^-16 of
+// themselves at most.  Larger ones (whose rounding would take the weights out
+// of their type's range in the end) by a difference first.
+constexpr float kFar = 256.f;
+
 // 32 query rows in one wave: lane % 32 is the row (its two half-waves hold
 // different keys of the scores and different dims of the sums).
 template <typename IO, int D>
@@ -249,7 +254,8 @@ struct Rows
 
     u4 q[kSteps];
     f16v o[kBlocks]; // sums, dims 32 i + 8 (e / 4) + 4 half + e % 4
-    float m;         // the largest score in use, times scale2
+    float m;         // the largest score in use, unscaled
+    bool far;        // some row's largest score is past kFar (wave-uniform)
     float l;         // this half-wave's part of the sum of weights
     int half, qi, head, hi_key, lo_key, sinks;
     float scale2;
@@ -276,6 +282,7 @@ struct Rows
             for (int e = 0; e < 16; e++)
                 o[i][e] = 0.f;
         m = kNegInf;
+        far = false;
         l = 0.f;
         const unsigned krow = lane & 31;
 #pragma unroll
@@ -346,7 +353,7 @@ struct Rows
             for (int e = 0; e < 16; e++)
                 s[i][e] = sees(key_of(k0, i, e)) ? s[i][e] : kNegInf;
     }
-    // scores to weights exp2(s scale2 - m), rounded for the product.  m is the
+    // scores to weights exp2((s - m) scale2), rounded for the product.  m is the
     // largest score but for a rise of up to kRise that the weights absorb; the
     // sums are rescaled when some row's maximum rises further (of 32 rows one
     // finds a larger score in nearly every tile: rescaling for each costs a
@@ -360,12 +367,13 @@ struct Rows
 #pragma unroll
             for (int e = 0; e < 16; e++)
                 top = fmaxf(top, s[i][e]);
-        top = partner_max(top) * scale2;
-        if (__builtin_amdgcn_ballot_w64(top - m > kRise) != 0)
+        top = partner_max(top);
+        if (__builtin_amdgcn_ballot_w64((top - m) * scale2 > kRise) != 0)
         {
             const float next = fmaxf(top, m);
-            const float alpha = next == kNegInf ? 1.f : __builtin_amdgcn_exp2f(m - next);
+            const float alpha = next == kNegInf ? 1.f : __builtin_amdgcn_exp2f((m - next) * scale2);
             m = next;
+            far = __builtin_amdgcn_ballot_w64(m != kNegInf && fabsf(m * scale2) > kFar) != 0;
             l *= alpha;
 #pragma unroll
             for (int i = 0; i < kBlocks; i++)
@@ -373,7 +381,17 @@ struct Rows
                 for (int e = 0; e < 16; e++)
                     o[i][e] *= alpha;
         }
-        const float base = m == kNegInf ? 0.f : m;
+        float base = m == kNegInf ? 0.f : m;
+        if (__builtin_expect(far, 0))
+        {
+#pragma unroll
+            for (int i = 0; i < NB; i++)
+#pragma unroll
+                for (int e = 0; e < 16; e++)
+                    s[i][e] -= base;
+            base = 0.f;
+        }
+        base *= scale2;
 #pragma unroll
         for (int i = 0; i < NB; i++)
 #pragma unroll
@@ -618,8 +636,8 @@ __global__ __launch_bounds__(64 * kWaves * GROUPS, 2) void slide_tile_kernel(Sli
         const float m = fmaxf(r.m, ml.x);
         const float base = m == kNegInf ? 0.f : m;
         // a group that saw no key of a row adds nothing
-        const float ca = r.m == kNegInf ? 0.f : __builtin_amdgcn_exp2f(r.m - base);
-        const float cb = ml.x == kNegInf ? 0.f : __builtin_amdgcn_exp2f(ml.x - base);
+        const float ca = r.m == kNegInf ? 0.f : __builtin_amdgcn_exp2f((r.m - base) * p.scale2);
+        const float cb = ml.x == kNegInf ? 0.f : __builtin_amdgcn_exp2f((ml.x - base) * p.scale2);
         r.m = m;
         r.l = r.l * ca + ml.y * cb;
 #pragma unroll
@@ -665,11 +683,11 @@ __global__ __launch_bounds__(64 * kWaves * GROUPS, 2) void slide_tile_kernel(Sli
             *reinterpret_cast<u2*>(dst + 64 * i + 16 * e) = l == 0.f ? u2{0u, 0u} : v; // no key: 0
         }
     if (p.lse && r.half == 0)
-        p.lse[to] = l == 0.f ? kNegInf : r.m * kLn2 + logf(l);
+        p.lse[to] = l == 0.f ? kNegInf : r.m * p.scale + logf(l);
 }
 
 // Few form, for at most 32 rows of a key head (single tokens): a stream of the
-// cache.  The four waves of a workgroup take tiles of 32 keys in turn, each
+// cache.  The two waves of a workgroup take tiles of 32 keys in turn, each
 // through LDS slots of its own with the next tiles on their way, so no barrier
 // stands in the stream; their sums are joined in LDS at the end.
 constexpr int kFewWaves = 2;
@@ -804,7 +822,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void slide_few_kernel(SlideParams p
         for (int w = 0; w < kFewWaves; w++)
             if (part[w].y != 0.f) // else it saw no key
             {
-                const float a = __builtin_amdgcn_exp2f(part[w].x - base);
+                const float a = __builtin_amdgcn_exp2f((part[w].x - base) * p.scale2);
                 const float4 u = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem + w * S::kWaveBytes) + rr * kPitch + d);
                 total += a * part[w].y;
                 v.x += a * u.x;
@@ -827,7 +845,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void slide_few_kernel(SlideParams p
         *reinterpret_cast<u2*>(p.out + at.b * p.o_b + qi * p.o_t + head * p.o_h + 2 * d) =
             total == 0.f ? u2{0u, 0u} : u2{IO::pack(v.x * inv, v.y * inv), IO::pack(v.z * inv, v.w * inv)};
         if (p.lse && d == 0)
-            p.lse[to] = total == 0.f ? kNegInf : m * kLn2 + logf(total);
+            p.lse[to] = total == 0.f ? kNegInf : m * p.scale + logf(total);
     }
 }
 
@@ -868,8 +886,8 @@ __global__ __launch_bounds__(32 * kTeams) void slide_join_kernel(SlideParams p, 
             {
                 const float next = fmaxf(m, ml[i].x);
                 const float base = next == kNegInf ? 0.f : next;
-                const float a = __builtin_amdgcn_exp2f(m - base);
-                const float c = __builtin_amdgcn_exp2f(ml[i].x - base);
+                const float a = __builtin_amdgcn_exp2f((m - base) * p.scale2);
+                const float c = __builtin_amdgcn_exp2f((ml[i].x - base) * p.scale2);
                 m = next;
                 l = l * a + c * ml[i].y;
                 o = o * a + c * v[i];
@@ -894,8 +912,8 @@ __global__ __launch_bounds__(32 * kTeams) void slide_join_kernel(SlideParams p, 
             continue;
         const float next = fmaxf(m, ml.x);
         const float base = next == kNegInf ? 0.f : next;
-        const float a = __builtin_amdgcn_exp2f(m - base);
-        const float c = __builtin_amdgcn_exp2f(ml.x - base);
+        const float a = __builtin_amdgcn_exp2f((m - base) * p.scale2);
+        const float c = __builtin_amdgcn_exp2f((ml.x - base) * p.scale2);
         m = next;
         l = l * a + c * ml.y;
         o = o * a + c * s_sum[team + t][lane];
@@ -909,13 +927,13 @@ __global__ __launch_bounds__(32 * kTeams) void slide_join_kernel(SlideParams p, 
     else
         *reinterpret_cast<unsigned*>(dst) = IO::pack(o[0] * inv, o[1] * inv);
     if (p.lse && lane == 0)
-        p.lse[at] = l == 0.f ? kNegInf : m * kLn2 + logf(l);
+        p.lse[at] = l == 0.f ? kNegInf : m * p.scale + logf(l);
 }
 
 // The form, and splits of the keys where the rows alone leave CUs without
-// work: two workgroups a CU at most in the tile form (two fit), three in the
-// few form (one fits at a time, and sequences of unlike lengths even out), two
-// tiles of keys each at least.
+// work: up to one workgroup a CU in the tile form (which then has two groups of
+// waves) with two tiles of keys each at least, up to two in the few form (two
+// fit) with a tile for each wave.
 void plan_tiles(SlideParams* p)
 {
     const long long rows = static_cast<long long>(p->q_len) * p->group;
@@ -945,7 +963,7 @@ int make_params(const sv2_sliding_attn_args* a, const char* what, SlideParams* o
         return bad("negative sizes, or heads not a multiple of kv_heads");
     if (a->left < 0 || a->right < 0 || a->sinks < 0)
         return bad("left, right and sinks must not be negative");
-    if (!(a->scale > 0.f) || !std::isfinite(a->scale))
+    if (!(a->scale > 0.f) || !std::isfinite(a->scale * kLog2e))
         return bad("scale must be positive and finite");
     if (a->dtype != SV2_F16 && a->dtype != SV2_BF16)
         return set_error(a->dtype == SV2_F32 ? SV2_EUNSUPPORTED : SV2_EINVAL, std::string(what) + ": dtype must be SV2_F16 or SV2_BF16");
@@ -965,6 +983,7 @@ int make_params(const sv2_sliding_attn_args* a, const char* what, SlideParams* o
     p.left = std::min(a->left, kMost);
     p.right = std::min(a->right, kMost - 1);
     p.sinks = std::min(a->sinks, kMost);
+    p.scale = a->scale;
     p.scale2 = a->scale * kLog2e;
     plan_tiles(&p);
     const long long tiles = static_cast<long long>(p.row_tiles) * p.kv_heads * p.batch;
@@ -1051,9 +1070,12 @@ try
         const int64_t s = strides[i];
         if (s < 0 || s % 8 != 0 || s > INT64_MAX / 4)
             return set_error(SV2_EINVAL, "sv2_sliding_attention: strides must be non-negative multiples of 8 elements");
+        if (i >= 9 && s == 0 && extents[i] > 1)
+            return set_error(SV2_EINVAL, "sv2_sliding_attention: a stride of out is 0");
     }
     // a tile's rows are addressed by 32-bit offsets from its first
-    constexpr int64_t kMostStride = INT32_MAX / (2 * kKeys) - 256;
+    constexpr int64_t kMostStride = 1 << 24;
+    static_assert((kKeys - 1) * 2 * kMostStride + 256 <= INT32_MAX, "offsets fit 32 bits");
     if (strides[4] > kMostStride || strides[7] > kMostStride)
         return set_error(SV2_EUNSUPPORTED, "sv2_sliding_attention: token stride of k or v above 2^24 elements");
     const long long need = workspace_of(p, a.head_dim);

@@ -382,7 +382,6 @@ def load() -> ctypes.CDLL:
     lib.sv2_sliding_attention.restype = i
     lib.sv2_group_norm_workspace.argtypes = [i, i, i, i, i]
     lib.sv2_group_norm_workspace.restype = ctypes.c_int64
-    i64 = ctypes.c_int64
     lib.sv2_group_norm.argtypes = [vp, i64, i64, vp, i64, i64, i, i, i, i, i, ctypes.c_float, vp, vp, i, vp,
                                    ctypes.c_size_t, vp]
     lib.sv2_group_norm.restype = i

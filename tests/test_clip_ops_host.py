@@ -123,3 +123,22 @@ def test_linear_nothing_to_do_and_null(hip):
     assert lib.sv2_linear(ctypes.byref(linear_args(hip, rows=0, x=None)), None) == 0
     assert lib.sv2_linear(ctypes.byref(linear_args(hip, out=0, y=None)), None) == 0
     assert lib.sv2_linear(None, None) == -1
+
+
+@pytest.mark.parametrize("over", [dict(out_token_stride=0), dict(out_head_stride=0), dict(out_batch_stride=0),
+                                  dict(scale=3e38)])
+def test_sliding_attention_refuses_outputs_that_coincide(hip, over):
+    """and a scale that is not finite in base 2."""
+    lib = hip.load()
+    assert lib.sv2_sliding_attention(ctypes.byref(sliding(hip, **over)), None) == -1
+    assert (b"scale" if "scale" in over else b"stride of out") in lib.sv2_last_error()
+
+
+def test_in_place_with_other_strides_is_refused(hip):
+    lib = hip.load()
+    for over in (dict(xr=72), dict(yr=72), dict(xi=0)):
+        assert lib.sv2_group_norm(*norm_args(hip, **over), None) == -1
+        assert b"y is x" in lib.sv2_last_error()
+    for over in (dict(y_stride=40), dict(residual_stride=40)):
+        assert lib.sv2_linear(ctypes.byref(linear_args(hip, **over)), None) == -1
+        assert b"residual is y" in lib.sv2_last_error()

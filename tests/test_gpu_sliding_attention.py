@@ -247,3 +247,40 @@ def test_streams_and_graph(hip, device):
         eager, _ = run(hip, q, k, v, 1900, 0, 8, kv_lens=kv)
         torch.cuda.synchronize()
         assert torch.equal(out, eager), n
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("nq,nk,h,d", [(1, 500, 4, 128), (1, 9000, 2, 64), (200, 700, 2, 128), (300, 300, 300, 64)])
+def test_scores_of_any_size(hip, device, nq, nk, h, d, dtype):
+    """Scores in the thousands and up to 2^40, products of powers of two and
+    small integers that fp32 holds: one key of each row carries all the weight,
+    or two equal ones share it, so out is their values (half the sum, rounded)
+    and lse the score."""
+    gen = torch.Generator(device=device).manual_seed(nk)
+    td = TD[dtype]
+    for power in (2.0 ** 12, 2.0 ** 20, 2.0 ** 32):
+        a = torch.randint(-120, 121, (nk,), generator=gen, device=device).float()
+        a[torch.randint(0, nk, (1,), generator=gen, device=device)] = 125.0
+        q = torch.zeros((1, nq, h, d), device=device)
+        k = torch.zeros((1, nk, h, d), device=device)
+        q[..., 0] = power ** 0.5
+        k[0, :, :, 0] = a[:, None] * power ** 0.5
+        v = torch.randn((1, nk, h, d), generator=gen, device=device).to(td)
+        q, k = q.to(td), k.to(td)
+        if not torch.isfinite(k).all():
+            assert td is torch.float16
+            k[0, :, :, 0] = a[:, None].to(td)
+            q[..., 0] = 2.0 ** 15
+        score = q[0, 0, 0, 0].double() * k[0, :, 0, 0].double()
+        out, lse = run(hip, q, k, v, nk, 0, 0, scale=4.0)
+        for i in range(nq):
+            seen = score[:nk - nq + i + 1]
+            top = torch.nonzero(seen == seen.max())[:, 0]
+            if len(top) > 2:
+                continue
+            # the mean of one or two values: exact in float64 and, but for the
+            # output's rounding, in fp32
+            want = v[0, top].double().mean(0).to(td)
+            assert torch.equal(out[0, i], want), (power, i)
+            far = 4.0 * float(seen.max()) + math.log(len(top))
+            assert (lse[0, :, i].double() - far).abs().max() <= abs(far) * 2.0 ** -22
