@@ -8,23 +8,23 @@
 // columns of one output row.
 //
 // Two forms, by the number of rows.
-//   few   up to 64 rows, and some blocks of 64 where these leave tiles few: a
-//         stream of w.  A workgroup of four waves takes 16 CT
+//   few   up to 64 rows (32 without alignment), and some blocks of 64 where these
+//         leave tiles few: a stream of w.  A workgroup of four waves takes 16 CT
 //         columns and splits K among its waves in blocks of 64 (interleaved:
 //         together they read 512 consecutive bytes of a row).  Each wave
 //         fetches whole 128-byte lines of w and x straight into a ring of LDS
 //         slots of its own, so no barrier stands in the stream; the four
 //         partial sums meet in LDS at the end.  One launch, no workspace.
-//   any   more rows whose operands the tile kernel of the inner products does
-//         not take: tiles through registers.
+//   any   operands that the tile kernel of the inner products does not take,
+//         from 33 rows or 4097 columns on: tiles through registers.
 //   tile  aligned operands of more rows: gemm.hip's persistent tiles.
 //
 // What they reach (MI355X): few, 1 x 2560 -> 15360 fp16 14 us (5.7 TB/s of w,
 // which the last-level cache holds in part), 58 x 5120 -> 2560 bf16 11 us (bound
 // by x: a workgroup brings 590 KB of it into LDS beside 160 of w);
-// any, 1999 x 1001 -> 777 with GELU and residual 26 us (16 steps, each a
+// any, 1999 x 1001 -> 777 with GELU and residual 22 us (16 steps, each a
 // barrier and LDS round trip for 416 workgroups of 4 waves), 16000 x 2561 ->
-// 2561 459 us (0.46 PFLOP/s); tile, 21658 x 2560 -> 6912 bf16 with bias and tanh
+// 2561 430 us (0.49 PFLOP/s); tile, 21658 x 2560 -> 6912 bf16 with bias and tanh
 // GELU 600 to 620 us (1.25 PFLOP/s; torch's product of these sizes alone 654).
 #include "sv2_internal.h"
 #include "activation.h"
@@ -81,11 +81,18 @@ struct LinearParams
 
 constexpr int kBK = 64; // K of a step: whole 128-byte lines of every row
 
-// 8 elements of a row from column k on, zeros past `k_end`.
+// 8 elements of a row from column k on, zeros past `k_end`: past the end, the
+// row's last 8 moved down.
 __device__ inline u4 load8(const uint16_t* row, int k, int k_end)
 {
-    if (k + 8 <= k_end)
-        return *reinterpret_cast<const u4u*>(row + k);
+    if (k_end >= 8)
+    {
+        const int at = min(k, k_end - 8);
+        const u4 v = *reinterpret_cast<const u4u*>(row + at);
+        const int gone = k - at;
+        const unsigned __int128 bits = __builtin_bit_cast(unsigned __int128, v);
+        return gone < 8 ? __builtin_bit_cast(u4, bits >> (16 * gone)) : u4{0u, 0u, 0u, 0u};
+    }
     u4 v = {0u, 0u, 0u, 0u};
 #pragma unroll
     for (int e = 0; e < 8; e++)
@@ -282,21 +289,34 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_few_kernel(LinearParams
             multiply();
     }
     // what the stream left: the last k of all (WHOLE), or everything
-    for (int k0 = done + 32 * wave; k0 < p.k; k0 += 32 * kFewWaves)
-    {
+    const uint16_t* wr[CT];
+    const uint16_t* xr[MT];
+#pragma unroll
+    for (int c = 0; c < CT; c++)
+        wr[c] = p.w + min(n0 + 16 * c + lr, p.n - 1) * p.ldw;
+#pragma unroll
+    for (int m = 0; m < MT; m++)
+        xr[m] = p.x + min(16 * m + lr, p.m - 1) * p.ldx;
+    auto pieces = [&](auto load, int k) {
         u4 a[CT], b[MT];
 #pragma unroll
         for (int c = 0; c < CT; c++)
-            a[c] = load8(p.w + min(n0 + 16 * c + lr, p.n - 1) * p.ldw, k0 + 8 * lq, p.k);
+            a[c] = load(wr[c], k);
 #pragma unroll
         for (int m = 0; m < MT; m++)
-            b[m] = load8(p.x + min(16 * m + lr, p.m - 1) * p.ldx, k0 + 8 * lq, p.k);
+            b[m] = load(xr[m], k);
 #pragma unroll
         for (int c = 0; c < CT; c++)
 #pragma unroll
             for (int m = 0; m < MT; m++)
                 acc[c][m] = IO::mfma(a[c], b[m], acc[c][m]);
-    }
+    };
+    int k0 = done + 32 * wave;
+#pragma unroll 4
+    for (; k0 + 32 <= p.k; k0 += 32 * kFewWaves)
+        pieces([](const uint16_t* row, int k) -> u4 { return *reinterpret_cast<const u4u*>(row + k); }, k0 + 8 * lq);
+    if (k0 < p.k)
+        pieces([&](const uint16_t* row, int k) { return load8(row, k, p.k); }, k0 + 8 * lq);
     // the waves' sums, added in wave order
     f4* sums = reinterpret_cast<f4*>(ring);
 #pragma unroll
@@ -326,9 +346,7 @@ struct AnyShape
     static constexpr int kOperand = TILE * kPitch;
     static constexpr int kLds = 2 * 2 * kOperand;
     static constexpr int kPieces = TILE * 8 / 256; // 16-byte pieces of an operand per thread and step
-    // steps held in registers: the small tiles' launches have few waves a CU
-    // to hide the loads' latency
-    static constexpr int kHeld = TILE == 128 ? 2 : 5;
+    static constexpr int kHeld = 2; // steps in registers (more: no faster, 1999 x 1001 -> 777 18.0 us, with five 19.8)
 };
 
 template <typename IO, int ACT, int TILE>
@@ -339,8 +357,13 @@ __global__ __launch_bounds__(256, TILE == 128 ? 2 : 3) void linear_any_kernel(Li
     constexpr int kPieces = S::kPieces;
     constexpr int kPart = TILE / 2; // of a wave, each way
     constexpr int kT = kPart / 16;
-    const int tn = blockIdx.x % p.tiles_n;
-    const int tm = blockIdx.x / p.tiles_n;
+    // XCD x (workgroup id mod 8) takes a contiguous run of tiles, which share
+    // rows of x in its L2
+    const int id = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+    const int tm = id / p.tiles_n;
+    const int tn = id - tm * p.tiles_n;
+    if (tm >= p.tiles_m)
+        return;
     const int m0 = tm * TILE;
     const int n0 = tn * TILE;
     const int lane = threadIdx.x & 63;
@@ -362,30 +385,20 @@ __global__ __launch_bounds__(256, TILE == 128 ? 2 : 3) void linear_any_kernel(Li
         xr[i] = p.x + min(m0 + cr + 32 * i, p.m - 1) * p.ldx;
         wr[i] = p.w + min(n0 + cr + 32 * i, p.n - 1) * p.ldw;
     }
-    const int steps = (p.k + kBK - 1) / kBK;
+    // whole steps; what K leaves follows them.  Loads stand in no branch: behind
+    // one, the wait for a step's loads would be one for all loads under way
+    const int steps = p.k / kBK;
     struct Held
     {
         u4 x[kPieces], w[kPieces];
     };
     auto load = [&](Held& h, int s) {
-        const int k = s * kBK + 8 * cc;
-        if ((s + 1) * kBK <= p.k)
-        {
+        const int k = min(s, steps - 1) * kBK + 8 * cc; // past the end: the last one again
 #pragma unroll
-            for (int i = 0; i < kPieces; i++)
-            {
-                h.x[i] = *reinterpret_cast<const u4u*>(xr[i] + k);
-                h.w[i] = *reinterpret_cast<const u4u*>(wr[i] + k);
-            }
-        }
-        else if (s < steps)
+        for (int i = 0; i < kPieces; i++)
         {
-#pragma unroll
-            for (int i = 0; i < kPieces; i++)
-            {
-                h.x[i] = load8(xr[i], k, p.k);
-                h.w[i] = load8(wr[i], k, p.k);
-            }
+            h.x[i] = *reinterpret_cast<const u4u*>(xr[i] + k);
+            h.w[i] = *reinterpret_cast<const u4u*>(wr[i] + k);
         }
     };
     auto put = [&](const Held& h, int s) {
@@ -422,30 +435,47 @@ __global__ __launch_bounds__(256, TILE == 128 ? 2 : 3) void linear_any_kernel(Li
                     acc[t][u] = IO::mfma(a[t], b[u], acc[t][u]);
         }
     };
-    // step s: the next one's registers go to LDS and are loaded again, for the
-    // step kHeld further
-    Held held[S::kHeld];
+    const bool rest = p.k % kBK != 0;
+    Held last;
+    if (rest)
 #pragma unroll
-    for (int i = 0; i < S::kHeld; i++)
-        load(held[i], i);
-    put(held[0], 0);
-    load(held[0], S::kHeld);
-    __syncthreads();
-    for (int s0 = 0; s0 < steps; s0 += S::kHeld)
-    {
-#pragma unroll
-        for (int u = 0; u < S::kHeld; u++)
+        for (int i = 0; i < kPieces; i++)
         {
-            const int s = s0 + u;
-            if (s >= steps)
-                break;
-            Held& h = held[(u + 1) % S::kHeld];
-            if (s + 1 < steps)
-                put(h, s + 1);
-            load(h, s + 1 + S::kHeld);
-            multiply(s);
-            __syncthreads();
+            last.x[i] = load8(xr[i], steps * kBK + 8 * cc, p.k);
+            last.w[i] = load8(wr[i], steps * kBK + 8 * cc, p.k);
         }
+    if (steps > 0)
+    {
+        // step s: the next one's registers go to LDS and are loaded again, for
+        // the step kHeld further
+        Held held[S::kHeld];
+#pragma unroll
+        for (int i = 0; i < S::kHeld; i++)
+            load(held[i], i);
+        put(held[0], 0);
+        load(held[0], S::kHeld);
+        __syncthreads();
+        for (int s0 = 0; s0 < steps; s0 += S::kHeld)
+        {
+#pragma unroll
+            for (int u = 0; u < S::kHeld; u++)
+            {
+                const int s = s0 + u;
+                if (s >= steps)
+                    break;
+                Held& h = held[(u + 1) % S::kHeld];
+                put(h, s + 1);
+                load(h, s + 1 + S::kHeld);
+                multiply(s);
+                __syncthreads();
+            }
+        }
+    }
+    if (rest)
+    {
+        put(last, 0);
+        __syncthreads();
+        multiply(0);
     }
 #pragma unroll
     for (int t = 0; t < kT; t++)
@@ -461,14 +491,15 @@ int run_any(LinearParams p, hipStream_t stream)
     p.tiles_m = (p.m + TILE - 1) / TILE;
     p.tiles_n = (p.n + TILE - 1) / TILE;
     const long long total = static_cast<long long>(p.tiles_m) * p.tiles_n;
-    if (total > INT_MAX)
+    if (total > INT_MAX - 8)
         return set_error(SV2_EUNSUPPORTED, "sv2_linear: too many tiles");
-    const int rc = set_dynamic_lds(reinterpret_cast<const void*>(&linear_any_kernel<IO, ACT, TILE>), AnyShape<TILE>::kLds,
+    constexpr int kLds = AnyShape<TILE>::kLds;
+    const int rc = set_dynamic_lds(reinterpret_cast<const void*>(&linear_any_kernel<IO, ACT, TILE>), kLds,
                                    "linear_any: dynamic LDS attribute");
     if (rc != SV2_OK)
         return rc;
-    hipLaunchKernelGGL((linear_any_kernel<IO, ACT, TILE>), dim3(static_cast<unsigned>(total)), dim3(256),
-                       AnyShape<TILE>::kLds, stream, p);
+    hipLaunchKernelGGL((linear_any_kernel<IO, ACT, TILE>), dim3((static_cast<unsigned>(total) + 7) / 8 * 8), dim3(256),
+                       kLds, stream, p);
     const hipError_t err = hipGetLastError();
     return err == hipSuccess ? SV2_OK : hip_error(err, "sv2_linear launch");
 }
@@ -476,11 +507,12 @@ int run_any(LinearParams p, hipStream_t stream)
 template <typename IO, int ACT>
 int run_linear(const LinearParams& p, hipStream_t stream)
 {
-    // the large tile where it gives every CU one: 2561 -> 2561 at 2000 rows (336
-    // tiles) 80 us in it and 100 in the small one, 4000 rows 148 and 175; 1001 ->
-    // 777 at 1999 rows (112) 33 and 20
+    // the large tile where it gives two thirds of the CUs one and its rows are
+    // not mostly empty: 2561 -> 2561 at 1200 rows (210 of them) 52 us in it and 72
+    // in the small one, at 2000 (336) 81 and 109, 1001 -> 777 at 3000 (168) 24.5
+    // and 23.8, at 1999 (112) 24 and 17
     const long long tiles = ((p.m + 127LL) / 128) * ((p.n + 127LL) / 128);
-    return tiles >= 256 ? run_any<IO, ACT, 128>(p, stream) : run_any<IO, ACT, 64>(p, stream);
+    return p.m > 64 && tiles >= 176 ? run_any<IO, ACT, 128>(p, stream) : run_any<IO, ACT, 64>(p, stream);
 }
 
 template <typename IO, int MT, int CT, bool WHOLE>
@@ -522,9 +554,9 @@ int run_few_rows(const LinearParams& p, hipStream_t stream)
 {
     if (p.m <= 16)
         return run_few<IO, 1, 1, WHOLE>(p, stream);
-    if (p.m <= 32)
+    if (!WHOLE || p.m <= 32)
         return run_few<IO, 2, 1, WHOLE>(p, stream);
-    return few_columns(p) == 4 ? run_few<IO, 4, 4, WHOLE>(p, stream) : run_few<IO, 4, 1, WHOLE>(p, stream);
+    return few_columns(p) == 4 ? run_few<IO, 4, 4, true>(p, stream) : run_few<IO, 4, 1, true>(p, stream);
 }
 
 template <typename IO>
@@ -597,7 +629,12 @@ try
     const bool tiles = linear_tiles_fit(o);
     // a few blocks of 64 rows stream faster than they fill tiles (2560 -> 2560
     // up to 384 rows, 640 -> 640 and 512 rows)
-    if (p.m <= kFewRows || (whole && tiles && p.m <= kFewMost && few_us(p, few_columns(p)) < linear_tiles_us(o)))
+    // rows that are not in whole pieces: the few form loads each where it is
+    // used, the tiles a step ahead (16 x 5001 -> 2001 26 us and 36, 24 x 1001 ->
+    // 777 8.4 and 11, but 60 x 5001 -> 2001 60 and 35, 16 x 2561 -> 15001, in
+    // rounds of workgroups, 65 and 26)
+    const bool few = whole ? p.m <= kFewRows : p.m <= 32 && p.n <= 16 * 256;
+    if (few || (whole && tiles && p.m <= kFewMost && few_us(p, few_columns(p)) < linear_tiles_us(o)))
     {
         if (a.dtype == SV2_F16)
             return whole ? run_few_rows<HalfIO, true>(p, st) : run_few_rows<HalfIO, false>(p, st);

@@ -1186,6 +1186,8 @@ def _enqueue(call, x, workspace, need, stream):
     dev = x.device
     if dev.type != "cuda":
         raise ValueError("tensors must be on a GPU")
+    if stream is not None and stream.device != dev:
+        raise ValueError(f"stream must be one of {dev}")
     if torch.cuda.current_device() != dev.index:
         with torch.cuda.device(dev):
             return _enqueue(call, x, workspace, need, stream)
@@ -1202,8 +1204,9 @@ def _enqueue(call, x, workspace, need, stream):
         ptr, size = workspace.data_ptr(), need
     else:
         ptr, size = None, 0
-    raw = torch._C._cuda_getCurrentRawStream(dev.index) if stream is None else stream.cuda_stream
-    return call(ptr, size, raw)
+    if stream is None:
+        return call(ptr, size, torch._C._cuda_getCurrentRawStream(dev.index))
+    return call(ptr, size, stream.cuda_stream)
 
 
 def _code(t):

@@ -142,3 +142,27 @@ def test_in_place_with_other_strides_is_refused(hip):
     for over in (dict(y_stride=40), dict(residual_stride=40)):
         assert lib.sv2_linear(ctypes.byref(linear_args(hip, **over)), None) == -1
         assert b"residual is y" in lib.sv2_last_error()
+
+
+def test_python_functions_refuse_tensors_that_do_not_fit(hip):
+    """By type, shape, layout and device, before any call into the library."""
+    import torch
+    h = torch.float16
+    q, k = torch.zeros((1, 2, 4, 64), dtype=h), torch.zeros((1, 9, 2, 64), dtype=h)
+    good = dict(q=q, k=k, v=k, out=torch.zeros_like(q), left=3)
+    for over in (dict(v=k[:, :8]), dict(k=k.bfloat16()), dict(out=q[:, :1]), dict(q=q.float()),
+                 dict(out=q.transpose(-1, -2).contiguous().transpose(-1, -2)),
+                 dict(kv_lens=torch.zeros(1, dtype=torch.int64)), dict(q_lens=torch.zeros(2, dtype=torch.int32)),
+                 dict(lse=torch.zeros((1, 2, 4))), dict()):  # the last: not on a GPU
+        with pytest.raises(ValueError):
+            hip.sliding_attention(**{**good, **over})
+    x = torch.zeros((2, 5, 8), dtype=h)
+    for more in (dict(y=x[:1]), dict(y=x.float()), dict(y=x.clone(), gamma=torch.zeros(8, dtype=h)),
+                 dict(y=x.clone(), beta=torch.zeros(7)), dict(y=x.double()), dict(y=x.clone())):
+        with pytest.raises(ValueError):
+            hip.group_norm(x, groups=2, **more)
+    w, y = torch.zeros((6, 8), dtype=h), torch.zeros((5, 6), dtype=h)
+    for over in (dict(w=w[:, :7]), dict(y=y[:4]), dict(x=x[0].float()), dict(residual=y[:, :5]), dict(bias=y[0]),
+                 dict(w=w.t().contiguous().t()), dict()):
+        with pytest.raises(ValueError):
+            hip.linear(**{**dict(x=x[0], w=w, y=y), **over})

@@ -93,3 +93,27 @@ def test_captured_layer_follows_its_inputs(hip, device):
         want = layer(hip, x, text).clone()
         torch.cuda.synchronize()
         assert torch.equal(got, want)
+
+
+def test_a_stream_that_is_not_current(hip, device):
+    """`stream=`: the work and its workspaces go there."""
+    gen = torch.Generator(device=device).manual_seed(3)
+    x = torch.randn((2, 9000, 64), generator=gen, device=device).to(torch.bfloat16)
+    w = torch.randn((64, 64), generator=gen, device=device).to(torch.bfloat16)
+    q = torch.randn((1, 1, 4, 128), generator=gen, device=device).to(torch.float16)
+    kv = torch.randn((1, 4000, 4, 128), generator=gen, device=device).to(torch.float16)
+
+    def calls(**more):
+        y, z, o = torch.zeros_like(x), torch.zeros_like(x[0]), torch.zeros_like(q)
+        torch.cuda.synchronize()
+        hip.group_norm(x, y, 8, activation=hip.ACT_GELU, **more)
+        hip.linear(y[1], w, z, **more)
+        hip.sliding_attention(q, kv, kv, o, left=3999, **more)
+        torch.cuda.synchronize()
+        return y, z, o
+
+    want = calls()
+    stream = torch.cuda.Stream()
+    for _ in range(3):
+        for a, b in zip(calls(stream=stream), want):
+            assert torch.equal(a, b)

@@ -154,3 +154,11 @@ def test_rows_past_4_gib(hip, device, m):
     torch.cuda.synchronize()
     want, tol = ex.linear(x, w, None, 0, None)
     ex.close(y, want, tol)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("k", [1, 7, 8, 9, 63, 64, 65, 128, 130, 191, 192, 201, 256])
+@pytest.mark.parametrize("m,n", [(20, 70), (33, 70), (20, 4100), (130, 70)])
+def test_ends_of_k_in_rows_without_alignment(hip, device, m, n, k, dtype):
+    """Whole steps, none of them, and every kind of rest."""
+    check(hip, device, m, k, n, TD[dtype], act=1, pad=3, shift=1)
