@@ -408,7 +408,8 @@ __global__ __launch_bounds__(kRowThreads, 4) void norm_stats_kernel(NormArgs p)
     float2* s_piece = reinterpret_cast<float2*>(smem); // [row lane][span of unit channels]
     for (int round = 0; round < k.rounds; round++)
     {
-        const int r0 = k.rounds > 1 ? 0 : quick_div(threadIdx.x, 1.f / static_cast<float>(k.nc));
+        // (quick_div here costs the large case 4 us of 188: its loop comes out differently)
+        const int r0 = k.rounds > 1 ? 0 : threadIdx.x / k.nc;
         const int col = k.rounds > 1 ? round * kRowThreads + threadIdx.x : threadIdx.x - r0 * k.nc;
         if (r0 >= k.lanes || col >= k.nc)
             continue;
