@@ -40,7 +40,7 @@
 //         its LDS reads; the two waves of a SIMD overlap them in part only
 //         (matrix unit 38% busy, vector unit 42%; 36% of a wave's time waiting
 //         to issue).  8250 tokens, window 2048, 20 heads
-//         of 128, bf16: 199 us, 0.78 PFLOP/s; 480 new tokens over 2400 of a
+//         of 128, bf16: 205 us, 0.76 PFLOP/s; 480 new tokens over 2400 of a
 //         cache 33 us, of which 27 this kernel.
 //         Tried and slower for that prompt: both products and the softmax of
 //         three successive tiles interleaved in one stream (235 us; 64 rows a
