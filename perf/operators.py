@@ -259,18 +259,12 @@ def _plain_linear(s):
 # ------------------------------------------------------- the library's own
 
 
-_sv2hip = None
-
-
 def _library():
-    """The package, imported once: a user's program does not look for it on
-    every call."""
-    global _sv2hip
-    if _sv2hip is None:
-        sys.path.insert(0, str(Path(__file__).resolve().parent.parent / "seedvr2-ncnn-valkan_amd"))
-        import sv2hip
-        _sv2hip = sv2hip
-    return _sv2hip
+    path = str(Path(__file__).resolve().parent.parent / "seedvr2-ncnn-valkan_amd")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    import sv2hip
+    return sv2hip
 
 
 def run(s):
