@@ -188,6 +188,14 @@ __device__ inline float partner_sum(float v)
     return a + b;
 }
 
+// sum * a, a >= 0 finite; a sum that is not finite stays as it is (a weight
+// too small for fp32 would make a NaN of an infinity).
+__device__ inline float rescaled(float sum, float a)
+{
+    const float x = sum * a;
+    return x == x ? x : sum;
+}
+
 // Four keys of one dim: within each 16-lane group such a read hands lane i
 // element i % 4 of the 8-byte pieces addressed by group lanes i / 4 + 4 j,
 // j = 0..3; when group lane k addresses key row r0 + k / 4 at dims
@@ -276,14 +284,7 @@ struct Rows
 #pragma unroll
         for (int c = 0; c < kSteps; c++)
             q[c] = *reinterpret_cast<const u4*>(qr + 32 * c);
-#pragma unroll
-        for (int i = 0; i < kBlocks; i++)
-#pragma unroll
-            for (int e = 0; e < 16; e++)
-                o[i][e] = 0.f;
-        m = kNegInf;
-        far = false;
-        l = 0.f;
+        restart();
         const unsigned krow = lane & 31;
 #pragma unroll
         for (int c = 0; c < kSteps; c++)
@@ -297,6 +298,30 @@ struct Rows
             const unsigned c = 4 * i + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
             voff[i] = vrow * kRowBytes + ((c ^ value_swz<D>(vrow)) << 4) + 8 * (lane & 1);
         }
+    }
+    __device__ void restart()
+    {
+#pragma unroll
+        for (int i = 0; i < kBlocks; i++)
+#pragma unroll
+            for (int e = 0; e < 16; e++)
+                o[i][e] = 0.f;
+        m = kNegInf;
+        far = false;
+        l = 0.f;
+    }
+    // Whether a sum of a row with a finite sum of weights is not finite: some
+    // value was not (wave-uniform).
+    __device__ bool odd() const
+    {
+        float t[4] = {0.f, 0.f, 0.f, 0.f}; // 0 or NaN
+#pragma unroll
+        for (int i = 0; i < kBlocks; i++)
+#pragma unroll
+            for (int e = 0; e < 16; e++)
+                t[e & 3] = __builtin_fmaf(o[i][e], 0.f, t[e & 3]);
+        const float any = (t[0] + t[1]) + (t[2] + t[3]);
+        return __builtin_amdgcn_ballot_w64(any != any && l == l) != 0;
     }
     // key of score e of key block i of a tile from key k0 on
     __device__ int key_of(int k0, int i, int e) const { return k0 + 4 * half + 32 * i + 8 * (e >> 2) + (e & 3); }
@@ -371,15 +396,25 @@ struct Rows
         if (__builtin_amdgcn_ballot_w64((top - m) * scale2 > kRise) != 0)
         {
             const float next = fmaxf(top, m);
-            const float alpha = next == kNegInf ? 1.f : __builtin_amdgcn_exp2f((m - next) * scale2);
+            // a row without a score so far holds zeros, or infinities
+            const float alpha = m == kNegInf ? 1.f : __builtin_amdgcn_exp2f((m - next) * scale2);
             m = next;
             far = __builtin_amdgcn_ballot_w64(m != kNegInf && fabsf(m * scale2) > kFar) != 0;
             l *= alpha;
+            if (__builtin_expect(__builtin_amdgcn_ballot_w64(alpha == 0.f) != 0, 0))
+            {
 #pragma unroll
-            for (int i = 0; i < kBlocks; i++)
+                for (int i = 0; i < kBlocks; i++)
 #pragma unroll
-                for (int e = 0; e < 16; e++)
-                    o[i][e] *= alpha;
+                    for (int e = 0; e < 16; e++)
+                        o[i][e] = rescaled(o[i][e], alpha);
+            }
+            else
+#pragma unroll
+                for (int i = 0; i < kBlocks; i++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++)
+                        o[i][e] *= alpha;
         }
         float base = m == kNegInf ? 0.f : m;
         if (__builtin_expect(far, 0))
@@ -421,10 +456,11 @@ struct Rows
             a[i] = values(vals, i, c);
     }
     // sums += weights values (`first`: the operands of the first 16 keys;
-    // `rest`: what the weights lack, if given); in a masked tile (from key k0
-    // on) values that are not finite stay out of the product
+    // `rest`: what the weights lack, if given) of the tile from key k0 on;
+    // `careful`: values that are not finite stay out of the product and are
+    // counted
     template <int NB>
-    __device__ void add(const u4 (&w)[2 * NB], u4 (&first)[kBlocks], const char* vals, int k0, bool masked,
+    __device__ void add(const u4 (&w)[2 * NB], u4 (&first)[kBlocks], const char* vals, int k0, bool careful,
                         const u4* rest = nullptr)
     {
         u4 next[kBlocks];
@@ -435,7 +471,7 @@ struct Rows
             if (c + 1 < 2 * NB)
                 read_values(c & 1 ? first : next, vals, c + 1);
             __builtin_amdgcn_sched_barrier(0);
-            if (masked)
+            if (careful)
             {
                 unsigned bad = 0;
 #pragma unroll
@@ -748,42 +784,58 @@ __global__ __launch_bounds__(64 * kFewWaves) void slide_few_kernel(SlideParams p
             dma16(vp, rr * v_step + ((c ^ value_swz<D>(r)) << 4), d + S::kTileBytes + j * 1024);
         }
     };
-    for (int i = 0; i < min(mine, S::kSlots - 1); i++)
-        fetch(i);
+    auto start = [&]() {
+        for (int i = 0; i < min(mine, S::kSlots - 1); i++)
+            fetch(i);
+    };
+    start();
     const int row = min(lane & 31, at.rows - 1);
     Rows<IO, D> r;
     r.init(p, at.b, at.kvh, row, at.off, at.nk, lane);
-    for (int i = 0; i < mine; i++)
+    // twice where a value is not finite: an infinity times the two terms of its
+    // weight is a NaN, so the second time such values are counted (looking for
+    // them in every tile costs 16 ragged caches 4 of 58 us)
+    bool careful = false;
+    for (;;)
     {
-        if (i + S::kSlots - 1 < mine)
+        for (int i = 0; i < mine; i++)
         {
-            // the slot worked on before is free once its reads are done
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            fetch(i + S::kSlots - 1);
-            wait_vm<(S::kSlots - 1) * 2 * kDma>();
+            if (i + S::kSlots - 1 < mine)
+            {
+                // the slot worked on before is free once its reads are done
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                fetch(i + S::kSlots - 1);
+                wait_vm<(S::kSlots - 1) * 2 * kDma>();
+            }
+            else
+                wait_vm<0>();
+            const int k0 = kt.key(t0 + wave + i * kFewWaves);
+            const char* st = ring + (i % S::kSlots) * 2 * S::kTileBytes;
+            const bool masked = is_masked(p, at.nk, p0, p1, k0, 32);
+            f16v s[1];
+            u4 w[2];
+            r.template scores<1>(s, st);
+            if (masked)
+                r.template mask<1>(s, k0);
+            u4 v0[Rows<IO, D>::kBlocks];
+            r.read_values(v0, st + S::kTileBytes, 0);
+            r.template weights<1>(s, w);
+            // their rounding errors
+            u4 rest[2];
+#pragma unroll
+            for (int c = 0; c < 2; c++)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    rest[c][e] = IO::pack(s[0][8 * c + 2 * e] - IO::to_float(w[c][e] & 0xffffu),
+                                          s[0][8 * c + 2 * e + 1] - IO::to_float(w[c][e] >> 16));
+            r.template add<1>(w, v0, st + S::kTileBytes, k0, masked || careful, rest);
         }
-        else
-            wait_vm<0>();
-        const int k0 = kt.key(t0 + wave + i * kFewWaves);
-        const char* st = ring + (i % S::kSlots) * 2 * S::kTileBytes;
-        const bool masked = is_masked(p, at.nk, p0, p1, k0, 32);
-        f16v s[1];
-        u4 w[2];
-        r.template scores<1>(s, st);
-        if (masked)
-            r.template mask<1>(s, k0);
-        u4 v0[Rows<IO, D>::kBlocks];
-        r.read_values(v0, st + S::kTileBytes, 0);
-        r.template weights<1>(s, w);
-        // their rounding errors
-        u4 rest[2];
-#pragma unroll
-        for (int c = 0; c < 2; c++)
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                rest[c][e] = IO::pack(s[0][8 * c + 2 * e] - IO::to_float(w[c][e] & 0xffffu),
-                                      s[0][8 * c + 2 * e + 1] - IO::to_float(w[c][e] >> 16));
-        r.template add<1>(w, v0, st + S::kTileBytes, k0, masked, rest);
+        if (careful || !r.odd())
+            break;
+        careful = true;
+        r.restart();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // the last tiles' slots are free
+        start();
     }
 
     // the waves' sums, relative to the largest maximum of a row
@@ -820,16 +872,16 @@ __global__ __launch_bounds__(64 * kFewWaves) void slide_few_kernel(SlideParams p
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < kFewWaves; w++)
-            if (part[w].y != 0.f) // else it saw no key
-            {
-                const float a = __builtin_amdgcn_exp2f((part[w].x - base) * p.scale2);
-                const float4 u = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem + w * S::kWaveBytes) + rr * kPitch + d);
-                total += a * part[w].y;
-                v.x += a * u.x;
-                v.y += a * u.y;
-                v.z += a * u.z;
-                v.w += a * u.w;
-            }
+        {
+            // of a wave that saw no score: 0
+            const float a = __builtin_amdgcn_exp2f((part[w].x - base) * p.scale2);
+            const float4 u = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem + w * S::kWaveBytes) + rr * kPitch + d);
+            total += a * part[w].y;
+            v.x += rescaled(u.x, a);
+            v.y += rescaled(u.y, a);
+            v.z += rescaled(u.z, a);
+            v.w += rescaled(u.w, a);
+        }
         const int qi = rr / p.group;
         const int head = at.kvh * p.group + (rr - qi * p.group);
         const long long to = (static_cast<long long>(at.b) * p.heads + head) * p.q_len + qi;
@@ -869,6 +921,18 @@ __global__ __launch_bounds__(32 * kTeams) void slide_join_kernel(SlideParams p, 
     float m = kNegInf;
     float l = 0.f;
     fe o = {};
+    // one part more; of one that saw no score the factor is 0
+    auto take = [&](float2 ml, fe v) {
+        const float next = fmaxf(m, ml.x);
+        const float base = next == kNegInf ? 0.f : next;
+        const float a = __builtin_amdgcn_exp2f((m - base) * p.scale2);
+        const float c = __builtin_amdgcn_exp2f((ml.x - base) * p.scale2);
+        m = next;
+        l = l * a + c * ml.y;
+#pragma unroll
+        for (int e = 0; e < kE; e++)
+            o[e] = rescaled(o[e], a) + rescaled(v[e], c);
+    };
     for (int s0 = mine; s0 < p.splits; s0 += 4 * per)
     {
         float2 ml[4];
@@ -882,16 +946,8 @@ __global__ __launch_bounds__(32 * kTeams) void slide_join_kernel(SlideParams p, 
         }
 #pragma unroll
         for (int i = 0; i < 4; i++)
-            if (s0 + i * per < p.splits && ml[i].y != 0.f) // else it saw no key
-            {
-                const float next = fmaxf(m, ml[i].x);
-                const float base = next == kNegInf ? 0.f : next;
-                const float a = __builtin_amdgcn_exp2f((m - base) * p.scale2);
-                const float c = __builtin_amdgcn_exp2f((ml[i].x - base) * p.scale2);
-                m = next;
-                l = l * a + c * ml[i].y;
-                o = o * a + c * v[i];
-            }
+            if (s0 + i * per < p.splits)
+                take(ml[i], v[i]);
     }
     s_sum[team][lane] = o;
     if (lane == 0)
@@ -906,18 +962,7 @@ __global__ __launch_bounds__(32 * kTeams) void slide_join_kernel(SlideParams p, 
     if (qi >= clamp_len(p.q_lens, b, p.q_len))
         return;
     for (int t = 1; t < per; t++)
-    {
-        const float2 ml = s_ml[team + t];
-        if (ml.y == 0.f)
-            continue;
-        const float next = fmaxf(m, ml.x);
-        const float base = next == kNegInf ? 0.f : next;
-        const float a = __builtin_amdgcn_exp2f((m - base) * p.scale2);
-        const float c = __builtin_amdgcn_exp2f((ml.x - base) * p.scale2);
-        m = next;
-        l = l * a + c * ml.y;
-        o = o * a + c * s_sum[team + t][lane];
-    }
+        take(s_ml[team + t], s_sum[team + t][lane]);
     if (l == 0.f)
         o = fe{}; // no key
     const float inv = l == 0.f ? 0.f : 1.f / l;
