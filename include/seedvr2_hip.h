@@ -611,7 +611,9 @@ typedef enum sv2_activation {
  * A query that sees no key gets 0 (lse -infinity); so does one whose visible
  * scores are all -infinity.  Rows i >= nq of out and lse are left as they
  * were.  Keys and values that no query of the sequence sees may hold
- * anything; what a query does not see does not reach its output. */
+ * anything; what a query does not see does not reach its output.  A visible
+ * value that is infinite or NaN does, in its dimension and whatever its weight
+ * (infinities of both signs: NaN). */
 typedef struct sv2_sliding_attn_args {
     int batch;
     int q_len, kv_len;   /* sizes of the token dimension of q / out and k / v */

@@ -27,7 +27,10 @@
 // Tiles of keys outside every row's window are not visited.  A tile in which
 // some row sees some key only is masked per element; there, values that are
 // not finite are kept out of the product (0 * Inf would poison the rows that
-// do not see them) and enter through products of indicators instead.
+// do not see them).  A value that is not finite is the sum of the rows that see
+// it, whatever its weight: where the tiles held one (or the sums show one), a
+// second walk over the tiles counts them by products of indicators (with one such
+// key the prompt below takes 268 us for 214).
 //
 // Forms, by the rows (heads of a key head x positions):
 //   few   up to 32 rows (single tokens): a stream of the cache, one row tile a
@@ -259,11 +262,13 @@ struct Rows
     static constexpr int kRowBytes = 2 * D;
     static constexpr int kSteps = D / 16;
     static constexpr int kBlocks = D / 32;
+    static constexpr unsigned kInf = IO::kExpMask & 0xffffu;
 
     u4 q[kSteps];
     f16v o[kBlocks]; // sums, dims 32 i + 8 (e / 4) + 4 half + e % 4
     float m;         // the largest score in use, unscaled
     bool far;        // some row's largest score is past kFar (wave-uniform)
+    bool found;      // a masked tile held a value that is not finite (wave-uniform)
     float l;         // this half-wave's part of the sum of weights
     int half, qi, head, hi_key, lo_key, sinks;
     float scale2;
@@ -284,7 +289,15 @@ struct Rows
 #pragma unroll
         for (int c = 0; c < kSteps; c++)
             q[c] = *reinterpret_cast<const u4*>(qr + 32 * c);
-        restart();
+#pragma unroll
+        for (int i = 0; i < kBlocks; i++)
+#pragma unroll
+            for (int e = 0; e < 16; e++)
+                o[i][e] = 0.f;
+        m = kNegInf;
+        far = false;
+        found = false;
+        l = 0.f;
         const unsigned krow = lane & 31;
 #pragma unroll
         for (int c = 0; c < kSteps; c++)
@@ -298,30 +311,6 @@ struct Rows
             const unsigned c = 4 * i + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
             voff[i] = vrow * kRowBytes + ((c ^ value_swz<D>(vrow)) << 4) + 8 * (lane & 1);
         }
-    }
-    __device__ void restart()
-    {
-#pragma unroll
-        for (int i = 0; i < kBlocks; i++)
-#pragma unroll
-            for (int e = 0; e < 16; e++)
-                o[i][e] = 0.f;
-        m = kNegInf;
-        far = false;
-        l = 0.f;
-    }
-    // Whether a sum of a row with a finite sum of weights is not finite: some
-    // value was not (wave-uniform).
-    __device__ bool odd() const
-    {
-        float t[4] = {0.f, 0.f, 0.f, 0.f}; // 0 or NaN
-#pragma unroll
-        for (int i = 0; i < kBlocks; i++)
-#pragma unroll
-            for (int e = 0; e < 16; e++)
-                t[e & 3] = __builtin_fmaf(o[i][e], 0.f, t[e & 3]);
-        const float any = (t[0] + t[1]) + (t[2] + t[3]);
-        return __builtin_amdgcn_ballot_w64(any != any && l == l) != 0;
     }
     // key of score e of key block i of a tile from key k0 on
     __device__ int key_of(int k0, int i, int e) const { return k0 + 4 * half + 32 * i + 8 * (e >> 2) + (e & 3); }
@@ -396,25 +385,15 @@ struct Rows
         if (__builtin_amdgcn_ballot_w64((top - m) * scale2 > kRise) != 0)
         {
             const float next = fmaxf(top, m);
-            // a row without a score so far holds zeros, or infinities
-            const float alpha = m == kNegInf ? 1.f : __builtin_amdgcn_exp2f((m - next) * scale2);
+            const float alpha = next == kNegInf ? 1.f : __builtin_amdgcn_exp2f((m - next) * scale2);
             m = next;
             far = __builtin_amdgcn_ballot_w64(m != kNegInf && fabsf(m * scale2) > kFar) != 0;
             l *= alpha;
-            if (__builtin_expect(__builtin_amdgcn_ballot_w64(alpha == 0.f) != 0, 0))
-            {
 #pragma unroll
-                for (int i = 0; i < kBlocks; i++)
+            for (int i = 0; i < kBlocks; i++)
 #pragma unroll
-                    for (int e = 0; e < 16; e++)
-                        o[i][e] = rescaled(o[i][e], alpha);
-            }
-            else
-#pragma unroll
-                for (int i = 0; i < kBlocks; i++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++)
-                        o[i][e] *= alpha;
+                for (int e = 0; e < 16; e++)
+                    o[i][e] *= alpha;
         }
         float base = m == kNegInf ? 0.f : m;
         if (__builtin_expect(far, 0))
@@ -455,12 +434,20 @@ struct Rows
         for (int i = 0; i < kBlocks; i++)
             a[i] = values(vals, i, c);
     }
+    // Whether an operand holds a value that is not finite: bit 15 or 31 set.
+    static __device__ unsigned bad_bits(u4 a)
+    {
+        unsigned bad = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            bad |= (a[e] & IO::kExpMask) + IO::kExpOne;
+        return bad & 0x80008000u;
+    }
     // sums += weights values (`first`: the operands of the first 16 keys;
-    // `rest`: what the weights lack, if given) of the tile from key k0 on;
-    // `careful`: values that are not finite stay out of the product and are
-    // counted
+    // `rest`: what the weights lack, if given); in a masked tile values that are
+    // not finite stay out of the product
     template <int NB>
-    __device__ void add(const u4 (&w)[2 * NB], u4 (&first)[kBlocks], const char* vals, int k0, bool careful,
+    __device__ void add(const u4 (&w)[2 * NB], u4 (&first)[kBlocks], const char* vals, bool masked,
                         const u4* rest = nullptr)
     {
         u4 next[kBlocks];
@@ -471,18 +458,25 @@ struct Rows
             if (c + 1 < 2 * NB)
                 read_values(c & 1 ? first : next, vals, c + 1);
             __builtin_amdgcn_sched_barrier(0);
-            if (careful)
+            if (masked)
             {
                 unsigned bad = 0;
 #pragma unroll
                 for (int i = 0; i < kBlocks; i++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        bad |= (a[i][e] & IO::kExpMask) + IO::kExpOne;
-                if (__builtin_expect(__builtin_amdgcn_ballot_w64((bad & 0x80008000u) != 0) != 0, 0))
+                    bad |= bad_bits(a[i]);
+                if (__builtin_expect(__builtin_amdgcn_ballot_w64(bad != 0) != 0, 0))
+                {
+                    found = true;
 #pragma unroll
                     for (int i = 0; i < kBlocks; i++)
-                        count_odd(a[i], key_of(k0, c >> 1, 8 * (c & 1)), o[i]);
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                        {
+                            const unsigned x = a[i][e];
+                            a[i][e] = ((x & kInf) == kInf ? 0u : x & 0xffffu) |
+                                      ((x >> 16 & kInf) == kInf ? 0u : x & 0xffff0000u);
+                        }
+                }
             }
 #pragma unroll
             for (int i = 0; i < kBlocks; i++)
@@ -493,13 +487,41 @@ struct Rows
                     o[i] = IO::mfma(a[i], rest[c], o[i]);
         }
     }
-    // Takes the values that are +Inf, -Inf or NaN out of an operand (of 16
-    // keys, this lane's from `first` on) and adds them to the sums of the rows
-    // that see one, by counting.
-    __device__ void count_odd(u4& a, int first, f16v& sum) const
+    // Whether some value was not finite (wave-uniform): a masked tile held one,
+    // or a sum is not, in a row whose weights are.
+    __device__ bool odd() const
     {
-        constexpr unsigned kInf = IO::kExpMask & 0xffffu;
-        asm volatile("" : "+v"(first)); // formed anew: kept, visibility outgrows the scalar registers
+        float t[4] = {0.f, 0.f, 0.f, 0.f}; // 0 or NaN
+#pragma unroll
+        for (int i = 0; i < kBlocks; i++)
+#pragma unroll
+            for (int e = 0; e < 16; e++)
+                t[e & 3] = __builtin_fmaf(o[i][e], 0.f, t[e & 3]);
+        const float any = (t[0] + t[1]) + (t[2] + t[3]);
+        return found || __builtin_amdgcn_ballot_w64(any != any && l == l) != 0;
+    }
+    // The values of a tile from key k0 on that are +Inf, -Inf or NaN, counted
+    // per row that sees them by products of indicators: they are the sums of
+    // those rows, whatever the weights (`given`, a bit a sum: one was there
+    // before).  A product with the weights makes a NaN of an infinity where a
+    // weight, or the second term of one, is 0 in 16 bits.
+    template <int NB>
+    __device__ void count(unsigned (&given)[kBlocks], const char* vals, int k0)
+    {
+        for (int c = 0; c < 2 * NB; c++)
+        {
+#pragma unroll
+            for (int i = 0; i < kBlocks; i++)
+            {
+                const u4 a = values(vals, i, c);
+                if (__builtin_amdgcn_ballot_w64(bad_bits(a) != 0) != 0)
+                    count_odd(a, key_of(k0, c >> 1, 8 * (c & 1)), o[i], given[i]);
+            }
+        }
+    }
+    // of one operand: 16 keys, this lane's from `first` on
+    __device__ void count_odd(u4 a, int first, f16v& sum, unsigned& given) const
+    {
 #pragma nounroll
         for (int kind = 0; kind < 3; kind++)
         {
@@ -524,13 +546,11 @@ struct Rows
             const float extra = kind == 0 ? -kNegInf : kind == 1 ? kNegInf : __builtin_nanf("");
 #pragma unroll
             for (int e = 0; e < 16; e++)
-                sum[e] = n[e] > 0.f ? sum[e] + extra : sum[e];
-        }
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-        {
-            a[e] = (a[e] & kInf) == kInf ? a[e] & 0xffff0000u : a[e];
-            a[e] = (a[e] >> 16 & kInf) == kInf ? a[e] & 0xffffu : a[e];
+                if (n[e] > 0.f)
+                {
+                    sum[e] = given >> e & 1 ? sum[e] + extra : extra;
+                    given |= 1u << e;
+                }
         }
     }
 };
@@ -647,7 +667,39 @@ __global__ __launch_bounds__(64 * kWaves * GROUPS, 2) void slide_tile_kernel(Sli
         u4 v0[Rows<IO, D>::kBlocks];
         r.read_values(v0, st + kTileBytes, 0);
         r.template weights<2>(s, w);
-        r.template add<2>(w, v0, st + kTileBytes, k0, masked);
+        r.template add<2>(w, v0, st + kTileBytes, masked);
+    }
+    bool again;
+    {
+        // where some wave met a value that is not finite, all go over the tiles
+        // again for these (the votes go through the buffers: their readers are
+        // done after the first barrier)
+        const bool odd = r.odd();
+        int* const votes = reinterpret_cast<int*>(smem);
+        bar();
+        if (lane == 0)
+            votes[kWaves * group + wave] = odd;
+        __syncthreads();
+        int all = 0;
+#pragma unroll
+        for (int i = 0; i < kWaves * GROUPS; i++)
+            all |= votes[i];
+        again = __builtin_amdgcn_readfirstlane(all) != 0;
+        if (__builtin_expect(again, 0))
+        {
+            unsigned given[kBlocks] = {};
+            bar(); // the votes are read
+            fetch(0);
+            for (int i = 0; i < steps; i++)
+            {
+                wait_vm<0>();
+                bar();
+                fetch(i + 1);
+                const int t = GROUPS * i + group;
+                if (GROUPS == 1 || t < nt)
+                    r.template count<2>(given, mine + (i & 1) * kBuf + kTileBytes, kt.key(t0 + t));
+            }
+        }
     }
     if constexpr (GROUPS > 1)
     {
@@ -671,22 +723,28 @@ __global__ __launch_bounds__(64 * kWaves * GROUPS, 2) void slide_tile_kernel(Sli
         const float2 ml = *give_ml;
         const float m = fmaxf(r.m, ml.x);
         const float base = m == kNegInf ? 0.f : m;
-        // a group that saw no key of a row adds nothing
-        const float ca = r.m == kNegInf ? 0.f : __builtin_amdgcn_exp2f((r.m - base) * p.scale2);
-        const float cb = ml.x == kNegInf ? 0.f : __builtin_amdgcn_exp2f((ml.x - base) * p.scale2);
+        // of a group that saw no score of a row: 0
+        const float ca = __builtin_amdgcn_exp2f((r.m - base) * p.scale2);
+        const float cb = __builtin_amdgcn_exp2f((ml.x - base) * p.scale2);
         r.m = m;
         r.l = r.l * ca + ml.y * cb;
+        auto join = [&](auto scaled) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < kBlocks; i++)
+            for (int i = 0; i < kBlocks; i++)
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-            {
-                const float4 v = give[(4 * i + e) * 64];
-                r.o[i][4 * e] = r.o[i][4 * e] * ca + v.x * cb;
-                r.o[i][4 * e + 1] = r.o[i][4 * e + 1] * ca + v.y * cb;
-                r.o[i][4 * e + 2] = r.o[i][4 * e + 2] * ca + v.z * cb;
-                r.o[i][4 * e + 3] = r.o[i][4 * e + 3] * ca + v.w * cb;
-            }
+                for (int e = 0; e < 4; e++)
+                {
+                    const float4 v = give[(4 * i + e) * 64];
+                    r.o[i][4 * e] = scaled(r.o[i][4 * e], ca) + scaled(v.x, cb);
+                    r.o[i][4 * e + 1] = scaled(r.o[i][4 * e + 1], ca) + scaled(v.y, cb);
+                    r.o[i][4 * e + 2] = scaled(r.o[i][4 * e + 2], ca) + scaled(v.z, cb);
+                    r.o[i][4 * e + 3] = scaled(r.o[i][4 * e + 3], ca) + scaled(v.w, cb);
+                }
+        };
+        if (again)
+            join([](float x, float c) { return rescaled(x, c); });
+        else
+            join([](float x, float c) { return x * c; });
     }
 
     const float l = partner_sum(r.l);
@@ -784,58 +842,55 @@ __global__ __launch_bounds__(64 * kFewWaves) void slide_few_kernel(SlideParams p
             dma16(vp, rr * v_step + ((c ^ value_swz<D>(r)) << 4), d + S::kTileBytes + j * 1024);
         }
     };
-    auto start = [&]() {
-        for (int i = 0; i < min(mine, S::kSlots - 1); i++)
-            fetch(i);
-    };
-    start();
+    for (int i = 0; i < min(mine, S::kSlots - 1); i++)
+        fetch(i);
     const int row = min(lane & 31, at.rows - 1);
     Rows<IO, D> r;
     r.init(p, at.b, at.kvh, row, at.off, at.nk, lane);
-    // twice where a value is not finite: an infinity times the two terms of its
-    // weight is a NaN, so the second time such values are counted (looking for
-    // them in every tile costs 16 ragged caches 4 of 58 us)
-    bool careful = false;
-    for (;;)
+    for (int i = 0; i < mine; i++)
     {
+        if (i + S::kSlots - 1 < mine)
+        {
+            // the slot worked on before is free once its reads are done
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            fetch(i + S::kSlots - 1);
+            wait_vm<(S::kSlots - 1) * 2 * kDma>();
+        }
+        else
+            wait_vm<0>();
+        const int k0 = kt.key(t0 + wave + i * kFewWaves);
+        const char* st = ring + (i % S::kSlots) * 2 * S::kTileBytes;
+        const bool masked = is_masked(p, at.nk, p0, p1, k0, 32);
+        f16v s[1];
+        u4 w[2];
+        r.template scores<1>(s, st);
+        if (masked)
+            r.template mask<1>(s, k0);
+        u4 v0[Rows<IO, D>::kBlocks];
+        r.read_values(v0, st + S::kTileBytes, 0);
+        r.template weights<1>(s, w);
+        // their rounding errors
+        u4 rest[2];
+#pragma unroll
+        for (int c = 0; c < 2; c++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                rest[c][e] = IO::pack(s[0][8 * c + 2 * e] - IO::to_float(w[c][e] & 0xffffu),
+                                      s[0][8 * c + 2 * e + 1] - IO::to_float(w[c][e] >> 16));
+        r.template add<1>(w, v0, st + S::kTileBytes, masked, rest);
+    }
+    if (__builtin_expect(r.odd(), 0)) // again, for the values that are not finite
+    {
+        unsigned given[kBlocks] = {};
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // the slots are free
         for (int i = 0; i < mine; i++)
         {
-            if (i + S::kSlots - 1 < mine)
-            {
-                // the slot worked on before is free once its reads are done
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                fetch(i + S::kSlots - 1);
-                wait_vm<(S::kSlots - 1) * 2 * kDma>();
-            }
-            else
-                wait_vm<0>();
-            const int k0 = kt.key(t0 + wave + i * kFewWaves);
-            const char* st = ring + (i % S::kSlots) * 2 * S::kTileBytes;
-            const bool masked = is_masked(p, at.nk, p0, p1, k0, 32);
-            f16v s[1];
-            u4 w[2];
-            r.template scores<1>(s, st);
-            if (masked)
-                r.template mask<1>(s, k0);
-            u4 v0[Rows<IO, D>::kBlocks];
-            r.read_values(v0, st + S::kTileBytes, 0);
-            r.template weights<1>(s, w);
-            // their rounding errors
-            u4 rest[2];
-#pragma unroll
-            for (int c = 0; c < 2; c++)
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    rest[c][e] = IO::pack(s[0][8 * c + 2 * e] - IO::to_float(w[c][e] & 0xffffu),
-                                          s[0][8 * c + 2 * e + 1] - IO::to_float(w[c][e] >> 16));
-            r.template add<1>(w, v0, st + S::kTileBytes, k0, masked || careful, rest);
+            fetch(i);
+            wait_vm<0>();
+            r.template count<1>(given, ring + (i % S::kSlots) * 2 * S::kTileBytes + S::kTileBytes,
+                                kt.key(t0 + wave + i * kFewWaves));
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
-        if (careful || !r.odd())
-            break;
-        careful = true;
-        r.restart();
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // the last tiles' slots are free
-        start();
     }
 
     // the waves' sums, relative to the largest maximum of a row

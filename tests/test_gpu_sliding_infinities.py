@@ -59,3 +59,62 @@ def test_few_rows_whose_weight_is_lost(hip, device, nq, nk, dtype):
     k[:, :nk // 2, :, 0] = -math.inf
     out, _ = run(hip, q, k, v, nk, 0, 0)
     assert (out[..., 3] == math.inf).all() and (out[..., 9] == -math.inf).all() and torch.isfinite(out[..., 20:39]).all()
+
+
+def lost(device, nq, nk, h, g, d, dtype):
+    """Scores so far apart that most weights are 0 in 16 bits, many in fp32:
+    small ones, a few large keys, and rising ones."""
+    q, k, v = make(device, 1, nq, nk, h, g, d, TD[dtype], seed=nk)
+    q, k = q.abs() + 0.5, k.abs() + 0.5
+    for far in (2.0, 8.0):
+        rise = torch.linspace(0, far, nk, device=device).to(k.dtype)[None, :, None, None]
+        yield q, k * rise, v.clone()
+        yield q, k * rise.flip(1), v.clone()
+    k = k * 0.125
+    k[:, 5::101] *= 16.0
+    yield q, k, v
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("nq,nk,h,g,d", [
+    (200, 1000, 2, 2, 128),   # two groups of waves, splits
+    (60, 6000, 2, 1, 64),     # many splits
+    (130, 700, 64, 64, 64),   # two groups, no split
+    (700, 900, 40, 40, 128),  # one group
+])
+def test_tiles_see_all(hip, device, nq, nk, h, g, d, dtype):
+    """Values of each kind at keys that every row sees, with weights that
+    matter and weights that are lost."""
+    at = (nk - nq) // 2
+    q, k, v = make(device, 1, nq, nk, h, g, d, TD[dtype])
+    plant(v, at)
+    out, _ = check(hip, q, k, v, nk, 0, 0)
+    assert (out[..., 3] == math.inf).all() and torch.isnan(out[..., 17]).all()
+    for q, k, v in lost(device, nq, nk, h, g, d, dtype):
+        plant(v, at)
+        plant(v, 8)
+        out, _ = check(hip, q, k, v, nk, 0, 0)
+        assert (out[..., 3] == math.inf).all() and (out[..., 9] == -math.inf).all() and torch.isnan(out[..., 17]).all()
+        # and where some rows see them only
+        plant(v, nk - nq + 20)
+        check(hip, q, k, v, nq // 2 + 100, 0, 12)
+
+
+@pytest.mark.parametrize("nq,h", [(150, 2), (700, 40)])
+def test_rows_that_are_not_finite_stay_alone(hip, device, nq, h):
+    """A row of NaN beside infinite values: its outputs are NaN, the others'
+    as they were."""
+    q, k, v = make(device, 1, nq, nq + 200, h, h, 64, torch.float16)
+    plain, _ = run(hip, q, k, v, 4000, 0, 0)
+    q2 = q.clone()
+    q2[0, 77, 1] = math.nan
+    out, _ = run(hip, q2, k, v, 4000, 0, 0)
+    assert torch.isnan(out[0, 77, 1]).all()
+    keep = torch.ones_like(out, dtype=torch.bool)
+    keep[0, 77, 1] = False
+    assert torch.equal(out[keep], plain[keep])
+    plant(v, 100)
+    out, _ = run(hip, q2, k, v, 4000, 0, 0)
+    assert torch.isnan(out[0, 77, 1]).all()
+    want, _ = check(hip, q, k, v, 4000, 0, 0)
+    assert torch.equal(out[keep].view(torch.int16), want[keep].view(torch.int16))
