@@ -588,7 +588,8 @@ int sv2_inner_product_f32(const float* x, const float* w, const float* bias, flo
  * dynamic_framewise_group_norm.cpp:62-143, with the activation that follows
  * it) and matrix products with their epilogues.  Strides are in elements;
  * the last dimension of every tensor is contiguous.  Outputs must not overlap
- * inputs except where said.
+ * inputs except where said.  Sizes that a launch cannot hold (2^32 threads)
+ * give SV2_EUNSUPPORTED.
  * ------------------------------------------------------------------------ */
 
 /* Activations, in fp32: v; v / (1 + exp(-v)); v/2 (1 + erf(v / sqrt 2));

@@ -1038,10 +1038,10 @@ int run_linear_rows(Form f, TileArgs a, int act, bool bf16, int r0, int rows, hi
     if (a.r)
         a.r += r0 * a.ldr;
     a.m = rows;
-    a.tiles_m = (rows + kCost[f].rows - 1) / kCost[f].rows;
-    a.tiles_n = (a.n + kCost[f].cols - 1) / kCost[f].cols;
+    a.tiles_m = static_cast<int>((rows + kCost[f].rows - 1LL) / kCost[f].rows);
+    a.tiles_n = static_cast<int>((a.n + kCost[f].cols - 1LL) / kCost[f].cols);
     const long long total = tiles_of(f, rows, a.n);
-    if (total > INT_MAX - kCus)
+    if (total > INT_MAX - kCus || (f == kSplit && !grid_fits(total + 7, kThreads)))
         return set_error(SV2_EUNSUPPORTED, "linear: too many tiles");
     a.total = static_cast<int>(total);
     a.group_m = 8;

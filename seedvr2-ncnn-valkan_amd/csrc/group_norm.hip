@@ -33,7 +33,6 @@
 #include "vec_io.h"
 
 #include <algorithm>
-#include <climits>
 #include <type_traits>
 
 namespace sv2
@@ -702,7 +701,7 @@ int run_norm(NormArgs p, int images, bool slab, const Slab& s, hipStream_t strea
         p.slab_groups = s.groups;
         p.slabs = (p.groups + s.groups - 1) / s.groups;
         const long long grid = static_cast<long long>(images) * p.slabs;
-        if (grid > INT_MAX - 8)
+        if (!grid_fits(grid + 7, s.threads))
             return set_error(SV2_EUNSUPPORTED, "sv2_group_norm: too many images");
         p.blocks = static_cast<int>(grid);
         const void* fn = reinterpret_cast<const void*>(&norm_slab_kernel<T, V, kKeep, ACT>);
@@ -716,7 +715,7 @@ int run_norm(NormArgs p, int images, bool slab, const Slab& s, hipStream_t strea
     {
         const long long grid = static_cast<long long>(images) * p.chunks;
         const long long joins = static_cast<long long>(images) * p.groups;
-        if (grid > INT_MAX || joins > INT_MAX)
+        if (!grid_fits(grid, kRowThreads) || !grid_fits(joins, kJoinThreads))
             return set_error(SV2_EUNSUPPORTED, "sv2_group_norm: too many images");
         const int lds = 2 * columns<V>(p.channels).lanes * p.channels * 4;
         const void* fn = reinterpret_cast<const void*>(&norm_stats_kernel<T, V>);

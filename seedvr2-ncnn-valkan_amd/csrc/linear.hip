@@ -31,7 +31,6 @@
 #include "vec_io.h"
 
 #include <algorithm>
-#include <climits>
 #include <cmath>
 
 namespace sv2
@@ -488,10 +487,10 @@ __global__ __launch_bounds__(256, TILE == 128 ? 2 : 3) void linear_any_kernel(Li
 template <typename IO, int ACT, int TILE>
 int run_any(LinearParams p, hipStream_t stream)
 {
-    p.tiles_m = (p.m + TILE - 1) / TILE;
-    p.tiles_n = (p.n + TILE - 1) / TILE;
+    p.tiles_m = static_cast<int>((p.m + TILE - 1LL) / TILE);
+    p.tiles_n = static_cast<int>((p.n + TILE - 1LL) / TILE);
     const long long total = static_cast<long long>(p.tiles_m) * p.tiles_n;
-    if (total > INT_MAX - 8)
+    if (!grid_fits(total + 7, 256))
         return set_error(SV2_EUNSUPPORTED, "sv2_linear: too many tiles");
     constexpr int kLds = AnyShape<TILE>::kLds;
     const int rc = set_dynamic_lds(reinterpret_cast<const void*>(&linear_any_kernel<IO, ACT, TILE>), kLds,
@@ -519,6 +518,8 @@ template <typename IO, int MT, int CT, bool WHOLE>
 int run_few(const LinearParams& p, hipStream_t stream)
 {
     constexpr int kLds = FewShape<MT, CT>::kLds;
+    if (!grid_fits((p.n + 16LL * CT - 1) / (16 * CT), 64 * kFewWaves))
+        return set_error(SV2_EUNSUPPORTED, "sv2_linear: too many columns");
     const int rc = set_dynamic_lds(reinterpret_cast<const void*>(&linear_few_kernel<IO, MT, CT, WHOLE>), kLds,
                                    "linear_few: dynamic LDS attribute");
     if (rc != SV2_OK)

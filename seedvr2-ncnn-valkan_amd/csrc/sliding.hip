@@ -1087,7 +1087,7 @@ int make_params(const sv2_sliding_attn_args* a, const char* what, SlideParams* o
     p.scale2 = a->scale * kLog2e;
     plan_tiles(&p);
     const long long tiles = static_cast<long long>(p.row_tiles) * p.kv_heads * p.batch;
-    if (tiles * p.splits > INT_MAX - 8)
+    if (!grid_fits(tiles * p.splits + 7, p.few ? 64 * kFewWaves : 64 * kWaves))
         return set_error(SV2_EUNSUPPORTED, std::string(what) + ": too many tiles");
     p.blocks = static_cast<int>(tiles * p.splits);
     *out = p;

@@ -199,6 +199,13 @@ bool gemm_mfma_preferred(int rows, int in, int out, int epi, const void* x, cons
 int gemm_mfma(hipStream_t stream, int rows, int in, int out, const void* x, const void* w, const void* w2, void* y,
               int epi, bool rounded, const float* bias, const float* gate, const void* residual);
 
+// Whether a launch of `blocks` workgroups of `threads` stays within the 2^32 - 1
+// threads of a grid's dimension.
+inline bool grid_fits(long long blocks, int threads)
+{
+    return blocks <= 0xffffffffLL / threads;
+}
+
 // The operands of sv2_linear: y = act(x W^T + bias) + r, strides in elements,
 // r and bias may be null.
 struct LinearOperands
