@@ -691,6 +691,19 @@ typedef struct sv2_linear_args {
  * of 8 elements run on the faster kernels.  Results do not depend on timing. */
 int sv2_linear(const sv2_linear_args* args, void* stream);
 
+/* Host.  How a call with these arguments runs; launches nothing and reads
+ * nothing behind the pointers (their alignment counts). */
+#define SV2_LINEAR_FEW 0   /* a stream of W, rows in blocks of 64 */
+#define SV2_LINEAR_ANY 1   /* tiles of any operands, through registers */
+#define SV2_LINEAR_TILES 2 /* tiles of aligned ones */
+typedef struct sv2_linear_form {
+    int kernel;     /* SV2_LINEAR_* */
+    int tile;       /* FEW: columns of a workgroup; ANY: rows and columns of one */
+    int first_rows; /* TILES: rows in 256 x 256 tiles, before the rest */
+    int form;       /* TILES: of the rest, SV2_FORM_* (else -1) */
+} sv2_linear_form;
+int sv2_linear_plan(const sv2_linear_args* args, sv2_linear_form* plan);
+
 /* ---- Euler sampler (src/model/sampler.h:18-78) and the latent preparation
  * of the engine loop (src/core/engine.cpp:79-149, :306-350).  Latents are
  * fp32 device arrays treated as flat element sequences except where a layout

@@ -1204,6 +1204,13 @@ double linear_tiles_us(const LinearOperands& o)
     return make_plan(o.m, o.k, o.n, kGemmLinear, false).us;
 }
 
+void linear_tiles_plan(const LinearOperands& o, int* first_rows, int* form)
+{
+    const Plan plan = make_plan(o.m, o.k, o.n, kGemmLinear, false);
+    *first_rows = plan.first_rows;
+    *form = plan.rest;
+}
+
 int linear_tiles(hipStream_t stream, const LinearOperands& o)
 {
     TileArgs a{};

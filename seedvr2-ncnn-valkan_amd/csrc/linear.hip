@@ -503,15 +503,20 @@ int run_any(LinearParams p, hipStream_t stream)
     return err == hipSuccess ? SV2_OK : hip_error(err, "sv2_linear launch");
 }
 
+// The any form's tile: the large one where it gives two thirds of the CUs one
+// and its rows are not mostly empty: 2561 -> 2561 at 1200 rows (210 of them) 52
+// us in it and 72 in the small one, at 2000 (336) 81 and 109, 1001 -> 777 at
+// 3000 (168) 24.5 and 23.8, at 1999 (112) 24 and 17
+int any_tile(const LinearParams& p)
+{
+    const long long tiles = ((p.m + 127LL) / 128) * ((p.n + 127LL) / 128);
+    return p.m > 64 && tiles >= 176 ? 128 : 64;
+}
+
 template <typename IO, int ACT>
 int run_linear(const LinearParams& p, hipStream_t stream)
 {
-    // the large tile where it gives two thirds of the CUs one and its rows are
-    // not mostly empty: 2561 -> 2561 at 1200 rows (210 of them) 52 us in it and 72
-    // in the small one, at 2000 (336) 81 and 109, 1001 -> 777 at 3000 (168) 24.5
-    // and 23.8, at 1999 (112) 24 and 17
-    const long long tiles = ((p.m + 127LL) / 128) * ((p.n + 127LL) / 128);
-    return p.m > 64 && tiles >= 176 ? run_any<IO, ACT, 128>(p, stream) : run_any<IO, ACT, 64>(p, stream);
+    return any_tile(p) == 128 ? run_any<IO, ACT, 128>(p, stream) : run_any<IO, ACT, 64>(p, stream);
 }
 
 template <typename IO, int MT, int CT, bool WHOLE>
@@ -544,10 +549,10 @@ double few_us(const LinearParams& p, int ct)
     return 1.5 + std::max({std::ceil(groups / 256) * round, 2e-6 * p.n * p.k / 5.0, x_us});
 }
 // Columns of a workgroup, in 16s: wide ones read x once for 64 columns and have
-// fewer workgroups (only worth it with x of more than 32 rows).
-int few_columns(const LinearParams& p)
+// fewer workgroups (only worth it with x of more than 32 rows in whole pieces).
+int few_columns(const LinearParams& p, bool whole)
 {
-    return p.m > 32 && few_us(p, 4) < few_us(p, 1) ? 4 : 1;
+    return whole && p.m > 32 && few_us(p, 4) < few_us(p, 1) ? 4 : 1;
 }
 
 template <typename IO, bool WHOLE>
@@ -557,7 +562,7 @@ int run_few_rows(const LinearParams& p, hipStream_t stream)
         return run_few<IO, 1, 1, WHOLE>(p, stream);
     if (!WHOLE || p.m <= 32)
         return run_few<IO, 2, 1, WHOLE>(p, stream);
-    return few_columns(p) == 4 ? run_few<IO, 4, 4, true>(p, stream) : run_few<IO, 4, 1, true>(p, stream);
+    return few_columns(p, true) == 4 ? run_few<IO, 4, 4, true>(p, stream) : run_few<IO, 4, 1, true>(p, stream);
 }
 
 template <typename IO>
@@ -590,19 +595,17 @@ int check_linear(const sv2_linear_args* a)
     return SV2_OK;
 }
 
-} // namespace
-} // namespace sv2
-
-extern "C" int sv2_linear(const sv2_linear_args* args, void* stream)
-try
+// A call of sv2_linear: its parameters and the kernel that takes it.
+struct LinearCall
 {
-    using namespace sv2;
-    const int rc = check_linear(args);
-    if (rc != SV2_OK)
-        return rc;
-    const sv2_linear_args& a = *args;
-    if (a.rows == 0 || a.out == 0)
-        return SV2_OK;
+    LinearParams p;
+    LinearOperands o;
+    bool whole; // x and w in pieces of 16 bytes, the rows a workgroup fetches within 32-bit offsets
+    int kernel; // SV2_LINEAR_*
+};
+
+int make_call(const sv2_linear_args& a, LinearCall* c)
+{
     if (!a.x || !a.w || !a.y)
         return set_error(SV2_EINVAL, "sv2_linear: null pointer");
     if (misaligned(a.x, 2) || misaligned(a.w, 2) || misaligned(a.y, 2) || misaligned(a.residual, 2) || misaligned(a.bias, 4))
@@ -621,31 +624,83 @@ try
     p.n = a.out;
     p.k = a.in;
     p.vec4 = p.n % 4 == 0 && p.ldy % 4 == 0 && p.ldr % 4 == 0 && !misaligned(p.y, 8) && !misaligned(p.r, 8);
-    const hipStream_t st = static_cast<hipStream_t>(stream);
     p.act = a.activation;
-    // pieces of 16 bytes: the rows a workgroup fetches lie within 32-bit offsets
-    const bool whole = p.ldx % 8 == 0 && p.ldw % 8 == 0 && !misaligned(p.x, 16) && !misaligned(p.w, 16) &&
-                       std::max(p.ldx, p.ldw) < (1LL << 31) / (2 * kFewRows);
-    const LinearOperands o{p.x, p.w, p.y, p.r, p.bias, p.ldx, p.ldw, p.ldy, p.ldr, p.m, p.n, p.k, p.act, a.dtype == SV2_BF16};
-    const bool tiles = linear_tiles_fit(o);
+    c->p = p;
+    c->o = LinearOperands{p.x, p.w, p.y, p.r, p.bias, p.ldx, p.ldw, p.ldy, p.ldr, p.m, p.n, p.k, p.act, a.dtype == SV2_BF16};
+    c->whole = p.ldx % 8 == 0 && p.ldw % 8 == 0 && !misaligned(p.x, 16) && !misaligned(p.w, 16) &&
+               std::max(p.ldx, p.ldw) < (1LL << 31) / (2 * kFewRows);
+    const bool tiles = linear_tiles_fit(c->o);
     // a few blocks of 64 rows stream faster than they fill tiles (2560 -> 2560
     // up to 384 rows, 640 -> 640 and 512 rows)
     // rows that are not in whole pieces: the few form loads each where it is
     // used, the tiles a step ahead (16 x 5001 -> 2001 26 us and 36, 24 x 1001 ->
     // 777 8.4 and 11, but 60 x 5001 -> 2001 60 and 35, 16 x 2561 -> 15001, in
     // rounds of workgroups, 65 and 26)
-    const bool few = whole ? p.m <= kFewRows : p.m <= 32 && p.n <= 16 * 256;
-    if (few || (whole && tiles && p.m <= kFewMost && few_us(p, few_columns(p)) < linear_tiles_us(o)))
+    const bool few = c->whole ? p.m <= kFewRows : p.m <= 32 && p.n <= 16 * 256;
+    if (few || (c->whole && tiles && p.m <= kFewMost && few_us(p, few_columns(p, true)) < linear_tiles_us(c->o)))
+        c->kernel = SV2_LINEAR_FEW;
+    else
+        c->kernel = tiles ? SV2_LINEAR_TILES : SV2_LINEAR_ANY;
+    return SV2_OK;
+}
+
+} // namespace
+} // namespace sv2
+
+extern "C" int sv2_linear(const sv2_linear_args* args, void* stream)
+try
+{
+    using namespace sv2;
+    const int rc = check_linear(args);
+    if (rc != SV2_OK)
+        return rc;
+    const sv2_linear_args& a = *args;
+    if (a.rows == 0 || a.out == 0)
+        return SV2_OK;
+    LinearCall c;
+    const int bad = make_call(a, &c);
+    if (bad != SV2_OK)
+        return bad;
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    const bool half = a.dtype == SV2_F16;
+    switch (c.kernel)
     {
-        if (a.dtype == SV2_F16)
-            return whole ? run_few_rows<HalfIO, true>(p, st) : run_few_rows<HalfIO, false>(p, st);
-        return whole ? run_few_rows<BfloatIO, true>(p, st) : run_few_rows<BfloatIO, false>(p, st);
+    case SV2_LINEAR_FEW:
+        if (half)
+            return c.whole ? run_few_rows<HalfIO, true>(c.p, st) : run_few_rows<HalfIO, false>(c.p, st);
+        return c.whole ? run_few_rows<BfloatIO, true>(c.p, st) : run_few_rows<BfloatIO, false>(c.p, st);
+    case SV2_LINEAR_TILES: return linear_tiles(st, c.o);
+    default: return half ? run_act<HalfIO>(c.p, a.activation, st) : run_act<BfloatIO>(c.p, a.activation, st);
     }
-    if (tiles)
-        return linear_tiles(st, o);
-    return a.dtype == SV2_F16 ? run_act<HalfIO>(p, a.activation, st) : run_act<BfloatIO>(p, a.activation, st);
 }
 catch (...)
 {
     return sv2::caught_exception("sv2_linear");
+}
+
+extern "C" int sv2_linear_plan(const sv2_linear_args* args, sv2_linear_form* plan)
+try
+{
+    using namespace sv2;
+    const int rc = check_linear(args);
+    if (rc != SV2_OK)
+        return rc;
+    if (!plan || args->rows == 0 || args->out == 0)
+        return set_error(SV2_EINVAL, "sv2_linear_plan: null plan or no outputs");
+    LinearCall c;
+    const int bad = make_call(*args, &c);
+    if (bad != SV2_OK)
+        return bad;
+    *plan = sv2_linear_form{c.kernel, 0, 0, -1};
+    switch (c.kernel)
+    {
+    case SV2_LINEAR_FEW: plan->tile = 16 * few_columns(c.p, c.whole); break;
+    case SV2_LINEAR_TILES: linear_tiles_plan(c.o, &plan->first_rows, &plan->form); break;
+    default: plan->tile = any_tile(c.p); break;
+    }
+    return SV2_OK;
+}
+catch (...)
+{
+    return sv2::caught_exception("sv2_linear_plan");
 }

@@ -226,6 +226,7 @@ constexpr int kGemmLinear = 3; // + sv2_activation: the tile kernel's epilogue c
 bool linear_tiles_fit(const LinearOperands& o);
 int linear_tiles(hipStream_t stream, const LinearOperands& o);
 double linear_tiles_us(const LinearOperands& o); // by the measured tile costs
+void linear_tiles_plan(const LinearOperands& o, int* first_rows, int* form); // SV2_FORM_*
 
 // fp16 y = epilogue(x W^T) for 1-64 rows on the weight-streaming kernel
 // (gemm_few.hip), the same epilogues as gemm_mfma (kGemmStore also takes an

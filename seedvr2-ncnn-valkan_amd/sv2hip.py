@@ -87,6 +87,7 @@ EXPORTS = [
     "sv2_group_norm_workspace",
     "sv2_group_norm",
     "sv2_linear",
+    "sv2_linear_plan",
     "sv2_euler_timesteps",
     "sv2_condition_ratio",
     "sv2_make_condition",
@@ -387,6 +388,8 @@ def load() -> ctypes.CDLL:
     lib.sv2_group_norm.restype = i
     lib.sv2_linear.argtypes = [ctypes.POINTER(LinearArgs), vp]
     lib.sv2_linear.restype = i
+    lib.sv2_linear_plan.argtypes = [ctypes.POINTER(LinearArgs), vp]
+    lib.sv2_linear_plan.restype = i
     lib.sv2_euler_timesteps.argtypes = [i, vp]
     lib.sv2_euler_timesteps.restype = i
     lib.sv2_condition_ratio.argtypes = [c_f, i, i, i]
@@ -1281,10 +1284,7 @@ def group_norm(x, y, groups, *, gamma=None, beta=None, eps=1e-5, activation=ACT_
     return y
 
 
-def linear(x, w, y, *, bias=None, activation=ACT_NONE, residual=None, stream=None):
-    """y = act(x W^T + bias) + residual (sv2_linear): x [rows, in], w [out, in],
-    y and residual [rows, out], all fp16 or all bf16 with contiguous rows; bias
-    fp32 [out].  y may be the residual."""
+def _linear_args(x, w, y, bias, activation, residual):
     import torch
     rows, k = x.shape
     n = w.shape[0]
@@ -1294,13 +1294,33 @@ def linear(x, w, y, *, bias=None, activation=ACT_NONE, residual=None, stream=Non
     _need("y", y, dtype, (rows, n), dev)
     if residual is not None:
         _need("residual", residual, dtype, (rows, n), dev)
-    a = LinearArgs(rows, k, n, _code(x), activation, x.data_ptr(), _row_step(x), w.data_ptr(), _row_step(w),
-                   _dense_ptr("bias", bias, torch.float32, (n,), dev),
-                   None if residual is None else residual.data_ptr(), 0 if residual is None else _row_step(residual),
-                   y.data_ptr(), _row_step(y))
+    return LinearArgs(rows, k, n, _code(x), activation, x.data_ptr(), _row_step(x), w.data_ptr(), _row_step(w),
+                      _dense_ptr("bias", bias, torch.float32, (n,), dev),
+                      None if residual is None else residual.data_ptr(), 0 if residual is None else _row_step(residual),
+                      y.data_ptr(), _row_step(y))
+
+
+def linear(x, w, y, *, bias=None, activation=ACT_NONE, residual=None, stream=None):
+    """y = act(x W^T + bias) + residual (sv2_linear): x [rows, in], w [out, in],
+    y and residual [rows, out], all fp16 or all bf16 with contiguous rows; bias
+    fp32 [out].  y may be the residual."""
+    a = _linear_args(x, w, y, bias, activation, residual)
     lib = load()
     check(_enqueue(lambda ptr, size, raw: lib.sv2_linear(ctypes.byref(a), raw), x, None, 0, stream), "sv2_linear")
     return y
+
+
+LINEAR_KERNELS = ("few", "any", "tiles")
+
+
+def linear_plan(x, w, y, *, bias=None, activation=ACT_NONE, residual=None):
+    """(kernel, tile, first_rows, form) of such a call of linear, by
+    sv2_linear_plan; nothing is launched.  A LinearArgs may stand for x, with w
+    and y None."""
+    a = x if isinstance(x, LinearArgs) else _linear_args(x, w, y, bias, activation, residual)
+    plan = (ctypes.c_int * 4)()
+    check(load().sv2_linear_plan(ctypes.byref(a), plan), "sv2_linear_plan")
+    return LINEAR_KERNELS[plan[0]], plan[1], plan[2], TILE_FORMS[plan[3]] if plan[3] >= 0 else None
 
 
 def sha256(data) -> bytes:
