@@ -583,7 +583,9 @@ int sv2_inner_product_f32(const float* x, const float* w, const float* bias, flo
 
 /* ------------------------------------------------------------------------
  * Operators around the DiT blocks for clips of many frames: attention of a
- * chunk of tokens over a cache, group normalisation of a channels-last video
+ * chunk of tokens over a cache (heads of 64 and 128; the reference's VAE
+ * attention, one head of 512, is not among them), group normalisation of a
+ * channels-last video
  * (the reference's DynamicFramewiseGroupNorm, src/layers/
  * dynamic_framewise_group_norm.cpp:62-143, with the activation that follows
  * it) and matrix products with their epilogues.  Strides are in elements;
@@ -614,7 +616,10 @@ typedef enum sv2_activation {
  * were.  Keys and values that no query of the sequence sees may hold
  * anything; what a query does not see does not reach its output.  A visible
  * value that is infinite or NaN does, in its dimension and whatever its weight
- * (infinities of both signs: NaN). */
+ * (infinities of both signs: NaN).
+ * Scores, maxima and sums are fp32.  With more than 32 query rows a key head
+ * (q_len heads / kv_heads) each softmax weight is rounded to dtype before it
+ * meets the values, which adds about as much as out's own rounding does. */
 typedef struct sv2_sliding_attn_args {
     int batch;
     int q_len, kv_len;   /* sizes of the token dimension of q / out and k / v */
@@ -668,12 +673,13 @@ int sv2_group_norm(const void* x, int64_t x_image_stride, int64_t x_row_stride, 
                    void* stream);
 
 /* y [rows, out] = act(x [rows, in] W^T + bias) + residual, W [out, in]; x, W,
- * y and residual of dtype, sums and bias in fp32, one rounding at the end.
+ * y and residual of dtype (fp16, bf16), sums and bias in fp32, one rounding at the end.
  * bias and residual may be NULL; y may be the residual with its stride
  * (another: SV2_EINVAL). */
 typedef struct sv2_linear_args {
     int rows, in, out; /* in at least 1 */
-    int dtype;      /* SV2_F16 or SV2_BF16 (fp32 products: sv2_inner_product_f32) */
+    int dtype;      /* SV2_F16 or SV2_BF16 (sv2_inner_product_f32 has fp32 products with a
+                       bias, without activation or residual) */
     int activation; /* sv2_activation */
     const void* x;
     int64_t x_stride; /* elements between rows, at least `in` */

@@ -438,8 +438,9 @@ __global__ __launch_bounds__(kRowThreads, 4) void norm_stats_kernel(NormArgs p)
                 for (int i = 0; i < kHeld; i++)
                     ahead[i].load(p.x, at + i * step);
             // sums of differences from the mean so far (the first row at the
-            // start): the subtraction below takes at most 7/8 of s2 away, the
-            // reference being one of the values or the mean of as many
+            // start): of kHeld rows the subtraction below takes at most
+            // (kHeld - 1) / kHeld of s2 away, 7/8 or 15/16, the reference being
+            // one of the values or the mean of as many
             float ref[V], s1[V], s2[V];
             if (done == 0)
                 h[0].get(mean);

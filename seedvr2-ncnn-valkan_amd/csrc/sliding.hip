@@ -17,7 +17,10 @@
 // types), which adds as much to the output's error as its own rounding does;
 // the sum of the weights is of the unrounded ones.  Where the cache's bytes
 // are the bound (the few form) P goes in as two such numbers, the second the
-// first one's rounding error: its products cost nothing there.
+// first one's rounding error: its products cost nothing there.  In the tile
+// form they cost 274 us for 215 at the prompt below, 39.5 for 33.5 at 480 new
+// tokens and 27.7 for 22.5 at head size 64, for an error against float64 of 1.0
+// times the output's own rounding in place of 1.35: one term there.
 //
 // A query row here is a (position, head) pair: the heads that share a key head
 // are packed into one tile of rows, position-major, so that a tile covers few
