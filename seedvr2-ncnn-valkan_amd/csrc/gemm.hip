@@ -65,8 +65,8 @@
 //                  strides, N and K not multiples of the tile: rows of W past
 //                  N repeat the last one and their sums are not stored, and
 //                  the last K % 64 of K go through registers once a tile.
-//                  21658 x 2560 -> 6912 bf16 with bias and tanh GELU: 600 to 640
-//                  us, 1.2 to 1.28 PFLOP/s; the matrix units are busy 62% of it.
+//                  21658 x 2560 -> 6912 bf16 with bias and tanh GELU: 600 to 650
+//                  us, 1.18 to 1.28 PFLOP/s; the matrix units are busy 62% of it.
 //                  One kernel an activation: a switch in one took 800 us.
 #include "sv2_internal.h"
 #include "activation.h"

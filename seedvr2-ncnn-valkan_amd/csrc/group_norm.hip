@@ -21,11 +21,12 @@
 //   rows   three launches: every workgroup reduces a run of rows, a small
 //          kernel joins the runs, and a last pass reads x again.
 //
-// What it reaches: 3 x 230400 x 256 bf16 with SiLU 184 us (rows form: 57 us of
-// statistics at 6.2 TB/s, 4 to join, 124 for the last pass at 5.7 TB/s, read and
-// write; one read and one write at a large copy's rate would be 142); 480 x 512
-// fp16 7.5 us (slab form, the latency of one launch); 3 x 3600 x 320 fp32 14 us
-// (three launches of 4 to 7).  Tried and taken back: image by image, so that the
+// What it reaches: 3 x 230400 x 256 bf16 with SiLU 185 us (rows form: 65 us of
+// statistics at 5.4 TB/s, 4 to join, 116 for the last pass at 6.1 TB/s, read and
+// write; one read and one write at a large copy's rate would be 142), with rows
+// of 264 elements 218, of 257 (one element a lane) 293; 480 x 512 fp16 7.5 us
+// (slab form, the latency of one launch); 3 x 3600 x 320 fp32 17 us (three
+// launches of 4 to 7).  Tried and taken back: image by image, so that the
 // last pass reads from the last-level cache (no faster, more launches); joining
 // in the last pass (15.6 us for the last case, 21 images 59 against 51).
 #include "sv2_internal.h"

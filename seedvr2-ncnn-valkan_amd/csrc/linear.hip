@@ -20,12 +20,13 @@
 //   tile  aligned operands of more rows: gemm.hip's persistent tiles.
 //
 // What they reach (MI355X): few, 1 x 2560 -> 15360 fp16 14 us (5.7 TB/s of w,
-// which the last-level cache holds in part), 58 x 5120 -> 2560 bf16 11 us (bound
+// which the last-level cache holds in part), 58 x 5120 -> 2560 bf16 11 to 12 us (bound
 // by x: a workgroup brings 590 KB of it into LDS beside 160 of w);
-// any, 1999 x 1001 -> 777 with GELU and residual 22 us (16 steps, each a
+// any, 1999 x 1001 -> 777 with GELU and residual 20 to 23 us (16 steps, each a
 // barrier and LDS round trip for 416 workgroups of 4 waves), 16000 x 2561 ->
 // 2561 430 us (0.49 PFLOP/s); tile, 21658 x 2560 -> 6912 bf16 with bias and tanh
-// GELU 600 to 620 us (1.25 PFLOP/s; torch's product of these sizes alone 654).
+// GELU 600 to 650 us by the card (1.18 to 1.28 PFLOP/s; torch's product of these
+// sizes alone 631 to 654).
 #include "sv2_internal.h"
 #include "activation.h"
 #include "vec_io.h"

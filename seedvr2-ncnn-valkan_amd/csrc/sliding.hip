@@ -39,18 +39,18 @@
 //   few   up to 32 rows (single tokens): a stream of the cache, one row tile a
 //         wave, the keys split over waves and workgroups.  Bound by the cache's
 //         bytes: sixteen tokens over 16 ragged caches, 227 MB of bf16 keys and
-//         values, 47 us (4.8 TB/s; a large copy reaches 5.0), 4.8 more to join
-//         the splits.
+//         values, 52 us (4.4 TB/s, two sets in turn; a large copy reaches 4.9),
+//         4.6 more to join the splits.
 //   tile  more rows: 128 of them a workgroup.  A tile of 64 keys is 32 matrix
 //         instructions a wave (1024 cycles) and about 220 vector ones beside
 //         its LDS reads; the two waves of a SIMD overlap them in part only
-//         (matrix unit 38% busy, vector unit 42%; 36% of a wave's time waiting
+//         (matrix unit 37% busy, vector unit 42%; 35% of a wave's time waiting
 //         to issue).  8250 tokens, window 2048, 20 heads
-//         of 128, bf16: 205 us, 0.76 PFLOP/s; 480 new tokens over 2400 of a
-//         cache 33 us, of which 27 this kernel.
+//         of 128, bf16: 214 us, 0.72 PFLOP/s; 480 new tokens over 2400 of a
+//         cache 34 us, of which 27 this kernel.
 //         Tried and slower for that prompt: both products and the softmax of
-//         three successive tiles interleaved in one stream (235 us; 64 rows a
-//         wave 392), eight waves in two groups a phase apart (257), wave
+//         three successive tiles interleaved in one stream (235 us beside 208;
+//         64 rows a wave 392), eight waves in two groups a phase apart (257), wave
 //         priorities (208 either way), the first rows last (215).
 //   join  where the keys were split: sums of a row in one team of lanes each.
 #include "sv2_internal.h"
