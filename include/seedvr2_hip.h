@@ -619,7 +619,9 @@ typedef enum sv2_activation {
  * (infinities of both signs: NaN).
  * Scores, maxima and sums are fp32.  With more than 32 query rows a key head
  * (q_len heads / kv_heads) each softmax weight is rounded to dtype before it
- * meets the values, which adds about as much as out's own rounding does. */
+ * meets the values, which adds about as much as out's own rounding does;
+ * weight_terms = 2 gives it a second number of dtype for what the first lacks
+ * and takes 1.2 to 1.3 times as long.  Fewer rows always have both. */
 typedef struct sv2_sliding_attn_args {
     int batch;
     int q_len, kv_len;   /* sizes of the token dimension of q / out and k / v */
@@ -641,6 +643,7 @@ typedef struct sv2_sliding_attn_args {
     float* lse;          /* device [batch][heads][q_len] or NULL: ln sum_j exp(scale q.k_j) */
     void* workspace;     /* device, sv2_sliding_attention_workspace() bytes; not shared by */
     size_t workspace_bytes; /* calls that may overlap */
+    int weight_terms;    /* 0 or 1: one, 2: two; the workspace is the same */
 } sv2_sliding_attn_args;
 
 /* Host.  Device workspace bytes of a call with these sizes (its pointers,

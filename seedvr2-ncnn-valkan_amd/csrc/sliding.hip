@@ -20,7 +20,8 @@
 // first one's rounding error: its products cost nothing there.  In the tile
 // form they cost 274 us for 215 at the prompt below, 39.5 for 33.5 at 480 new
 // tokens and 27.7 for 22.5 at head size 64, for an error against float64 of 1.0
-// times the output's own rounding in place of 1.35: one term there.
+// times the output's own rounding in place of 1.35: the caller's choice there,
+// one term unless it asks for two.
 //
 // A query row here is a (position, head) pair: the heads that share a key head
 // are packed into one tile of rows, position-major, so that a tile covers few
@@ -127,6 +128,7 @@ struct SlideParams
     int batch, q_len, kv_len, heads, kv_heads, group;
     int left, right, sinks;
     int few, row_tiles, splits, blocks;
+    int terms; // of a weight in the tile form
 };
 
 constexpr int kKeys = 64;      // keys of a tile
@@ -423,6 +425,17 @@ struct Rows
             for (int e = 0; e < 4; e++)
                 w[c][e] = IO::pack(s[c >> 1][8 * (c & 1) + 2 * e], s[c >> 1][8 * (c & 1) + 2 * e + 1]);
     }
+    // what the rounded weights lack: their second terms
+    template <int NB>
+    static __device__ void rounding_of(const f16v (&s)[NB], const u4 (&w)[2 * NB], u4 (&rest)[2 * NB])
+    {
+#pragma unroll
+        for (int c = 0; c < 2 * NB; c++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                rest[c][e] = IO::pack(s[c >> 1][8 * (c & 1) + 2 * e] - IO::to_float(w[c][e] & 0xffffu),
+                                      s[c >> 1][8 * (c & 1) + 2 * e + 1] - IO::to_float(w[c][e] >> 16));
+    }
     // values of keys 16 c .. 16 c + 15 of a tile, dims 32 i on
     __device__ u4 values(const char* vals, int i, int c) const
     {
@@ -593,7 +606,8 @@ struct Place
 // GROUPS = 2, for launches that give a CU one workgroup at most: a second
 // group of four waves takes every other tile for the same rows, and its sums
 // are joined to the first's in LDS.
-template <typename IO, int D, int GROUPS>
+// TERMS: 16-bit numbers that a weight goes into the product as.
+template <typename IO, int D, int GROUPS, int TERMS>
 __global__ __launch_bounds__(64 * kWaves * GROUPS, 2) void slide_tile_kernel(SlideParams p)
 {
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -670,7 +684,14 @@ __global__ __launch_bounds__(64 * kWaves * GROUPS, 2) void slide_tile_kernel(Sli
         u4 v0[Rows<IO, D>::kBlocks];
         r.read_values(v0, st + kTileBytes, 0);
         r.template weights<2>(s, w);
-        r.template add<2>(w, v0, st + kTileBytes, masked);
+        if constexpr (TERMS == 2)
+        {
+            u4 rest[4];
+            r.template rounding_of<2>(s, w, rest);
+            r.template add<2>(w, v0, st + kTileBytes, masked, rest);
+        }
+        else
+            r.template add<2>(w, v0, st + kTileBytes, masked);
     }
     bool again;
     {
@@ -872,14 +893,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void slide_few_kernel(SlideParams p
         u4 v0[Rows<IO, D>::kBlocks];
         r.read_values(v0, st + S::kTileBytes, 0);
         r.template weights<1>(s, w);
-        // their rounding errors
         u4 rest[2];
-#pragma unroll
-        for (int c = 0; c < 2; c++)
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                rest[c][e] = IO::pack(s[0][8 * c + 2 * e] - IO::to_float(w[c][e] & 0xffffu),
-                                      s[0][8 * c + 2 * e + 1] - IO::to_float(w[c][e] >> 16));
+        r.template rounding_of<1>(s, w, rest);
         r.template add<1>(w, v0, st + S::kTileBytes, masked, rest);
     }
     if (__builtin_expect(r.odd(), 0)) // again, for the values that are not finite
@@ -1072,6 +1087,8 @@ int make_params(const sv2_sliding_attn_args* a, const char* what, SlideParams* o
         return set_error(a->dtype == SV2_F32 ? SV2_EUNSUPPORTED : SV2_EINVAL, std::string(what) + ": dtype must be SV2_F16 or SV2_BF16");
     if (a->head_dim != 64 && a->head_dim != 128)
         return set_error(SV2_EUNSUPPORTED, std::string(what) + ": head_dim must be 64 or 128");
+    if (a->weight_terms < 0 || a->weight_terms > 2)
+        return bad("weight_terms must be 0, 1 or 2");
     constexpr int kMost = 1 << 30;
     if (a->q_len > kMost / a->heads || a->kv_len > kMost)
         return set_error(SV2_EUNSUPPORTED, std::string(what) + ": more than 2^30 query rows or keys");
@@ -1088,6 +1105,7 @@ int make_params(const sv2_sliding_attn_args* a, const char* what, SlideParams* o
     p.sinks = std::min(a->sinks, kMost);
     p.scale = a->scale;
     p.scale2 = a->scale * kLog2e;
+    p.terms = std::max(1, a->weight_terms);
     plan_tiles(&p);
     const long long tiles = static_cast<long long>(p.row_tiles) * p.kv_heads * p.batch;
     if (!grid_fits(tiles * p.splits + 7, p.few ? 64 * kFewWaves : 64 * kWaves))
@@ -1108,9 +1126,10 @@ int run_slide(const SlideParams& p, hipStream_t stream)
     const int groups = p.blocks <= 256 ? 2 : 1; // one workgroup a CU: twice the waves
     const int lds = p.few ? FewShape<D>::kLds : groups * 2 * 2 * kKeys * 2 * D;
     const int threads = 64 * (p.few ? kFewWaves : kWaves * groups);
-    auto kernel = p.few         ? &slide_few_kernel<IO, D>
-                  : groups == 2 ? &slide_tile_kernel<IO, D, 2>
-                                : &slide_tile_kernel<IO, D, 1>;
+    auto kernel = p.few          ? &slide_few_kernel<IO, D>
+                  : p.terms == 2 ? (groups == 2 ? &slide_tile_kernel<IO, D, 2, 2> : &slide_tile_kernel<IO, D, 1, 2>)
+                  : groups == 2  ? &slide_tile_kernel<IO, D, 2, 1>
+                                 : &slide_tile_kernel<IO, D, 1, 1>;
     const int rc = set_dynamic_lds(reinterpret_cast<const void*>(kernel), lds, "sv2_sliding_attention: dynamic LDS attribute");
     if (rc != SV2_OK)
         return rc;

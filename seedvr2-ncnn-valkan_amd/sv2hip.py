@@ -154,7 +154,7 @@ class SlidingAttnArgs(ctypes.Structure):
             (x, ctypes.c_void_p), (x + "_batch_stride", ctypes.c_int64), (x + "_token_stride", ctypes.c_int64),
             (x + "_head_stride", ctypes.c_int64))]
         + [("q_lens", ctypes.c_void_p), ("kv_lens", ctypes.c_void_p), ("lse", ctypes.c_void_p),
-           ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)])
+           ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t), ("weight_terms", ctypes.c_int)])
 
 
 class LinearArgs(ctypes.Structure):
@@ -1224,15 +1224,16 @@ def _code(t):
 
 
 def sliding_attention(q, k, v, out, *, left, right=0, sinks=0, scale=None, q_lens=None, kv_lens=None, lse=None,
-                      workspace=None, stream=None):
+                      weight_terms=1, workspace=None, stream=None):
     """Attention of q [batch, q_len, heads, dim] over a cache k, v [batch,
     kv_len, kv_heads, dim] with a sliding window and first tokens that stay
     visible (sv2_sliding_attention), into `out` (as q) and `lse` [batch, heads,
     q_len] fp32 when given.  The query of token i of a sequence stands at p =
     kv_len - q_len + i and sees the keys j <= p + right with j < sinks or j >=
     p - left; `q_lens`, `kv_lens`: int32 device tensors [batch] of each
-    sequence's own lengths.  `scale`: dim ** -0.5 when None.  Tensors may be
-    strided views with a contiguous last dimension."""
+    sequence's own lengths.  `scale`: dim ** -0.5 when None.  `weight_terms`: 2
+    keeps the softmax weights of more than 32 rows a key head from being rounded
+    to 16 bits.  Tensors may be strided views with a contiguous last dimension."""
     import torch
     shape = q.shape
     b, nq, h, d = shape
@@ -1246,7 +1247,7 @@ def sliding_attention(q, k, v, out, *, left, right=0, sinks=0, scale=None, q_len
                         *_need("v", v, dtype, cache, dev), *_need("out", out, dtype, shape, dev),
                         _dense_ptr("q_lens", q_lens, torch.int32, (b,), dev),
                         _dense_ptr("kv_lens", kv_lens, torch.int32, (b,), dev),
-                        _dense_ptr("lse", lse, torch.float32, (b, h, nq), dev))
+                        _dense_ptr("lse", lse, torch.float32, (b, h, nq), dev), None, 0, weight_terms)
     lib = load()
     ref = ctypes.byref(a)
     need = lib.sv2_sliding_attention_workspace(ref)
